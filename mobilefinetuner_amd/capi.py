@@ -31,6 +31,14 @@ EXPORTS = (
     "mft_lm_ce_streaming_bwd",
     "mft_lora_workspace_size", "mft_lora_fwd", "mft_lora_bwd", "mft_lora_merge",
 )
+# The same of the layers around attention: layer_norm.h, linear.h and logprobs.h.
+LAYER_EXPORTS = (
+    "mft_layer_norm_fwd", "mft_layer_norm_workspace_size", "mft_layer_norm_bwd",
+    "mft_linear_workspace_size", "mft_linear_fwd", "mft_linear_bwd",
+    "mft_logprobs_workspace_size", "mft_logprobs_fwd", "mft_logprobs_bwd",
+)
+LOGPROBS_MAX_TOP = 64
+MFT_ACT_NONE, MFT_ACT_RELU, MFT_ACT_GELU_TANH, MFT_ACT_SILU = 0, 1, 2, 3
 MFT_REDUCE_MEAN, MFT_REDUCE_SUM, MFT_REDUCE_NONE = 0, 1, 2
 
 
@@ -78,6 +86,21 @@ class LoraDesc(C.Structure):
     _fields_ = [("N", C.c_int64), ("in_dim", C.c_int64), ("out_dim", C.c_int64), ("w_dtype", C.c_int32),
                 ("w_transposed", C.c_int32), ("n_slices", C.c_int32), ("grads_for_column_slices", C.c_int32),
                 ("slices", C.POINTER(LoraSlice))]
+
+
+class LayerNormDesc(C.Structure):
+    _fields_ = [("N", C.c_int64), ("D", C.c_int64), ("dtype", C.c_int32), ("eps", C.c_float)] + \
+        [(n, C.c_int64) for n in ("x_stride", "y_stride", "dy_stride", "dx_stride")]
+
+
+class LinearDesc(C.Structure):
+    _fields_ = [("N", C.c_int64), ("in_dim", C.c_int64), ("out_dim", C.c_int64), ("dtype", C.c_int32),
+                ("w_transposed", C.c_int32), ("activation", C.c_int32)]
+
+
+class LogprobsDesc(C.Structure):
+    _fields_ = [("N", C.c_int64), ("V", C.c_int64), ("ld", C.c_int64), ("grad_ld", C.c_int64), ("dtype", C.c_int32),
+                ("ignore_index", C.c_int32), ("top", C.c_int32)]
 
 
 class MftError(RuntimeError):
@@ -146,6 +169,24 @@ def lib():
     L.mft_lora_bwd.argtypes = [C.POINTER(LoraDesc)] + [vp] * 7
     L.mft_lora_merge.restype = C.c_int
     L.mft_lora_merge.argtypes = [C.POINTER(LoraDesc), vp, C.c_float, vp]
+    L.mft_layer_norm_fwd.restype = C.c_int
+    L.mft_layer_norm_fwd.argtypes = [C.POINTER(LayerNormDesc)] + [vp] * 7
+    L.mft_layer_norm_workspace_size.restype = C.c_int
+    L.mft_layer_norm_workspace_size.argtypes = [C.POINTER(LayerNormDesc), C.POINTER(C.c_size_t)]
+    L.mft_layer_norm_bwd.restype = C.c_int
+    L.mft_layer_norm_bwd.argtypes = [C.POINTER(LayerNormDesc)] + [vp] * 10
+    L.mft_linear_workspace_size.restype = C.c_int
+    L.mft_linear_workspace_size.argtypes = [C.POINTER(LinearDesc), C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]
+    L.mft_linear_fwd.restype = C.c_int
+    L.mft_linear_fwd.argtypes = [C.POINTER(LinearDesc)] + [vp] * 8
+    L.mft_linear_bwd.restype = C.c_int
+    L.mft_linear_bwd.argtypes = [C.POINTER(LinearDesc)] + [vp] * 9
+    L.mft_logprobs_workspace_size.restype = C.c_int
+    L.mft_logprobs_workspace_size.argtypes = [C.POINTER(LogprobsDesc), C.POINTER(C.c_size_t)]
+    L.mft_logprobs_fwd.restype = C.c_int
+    L.mft_logprobs_fwd.argtypes = [C.POINTER(LogprobsDesc)] + [vp] * 10
+    L.mft_logprobs_bwd.restype = C.c_int
+    L.mft_logprobs_bwd.argtypes = [C.POINTER(LogprobsDesc)] + [vp] * 8
     if L.mft_version() != 7:
         raise RuntimeError("libmft_attn.so version mismatch")
     _lib = L
@@ -324,3 +365,60 @@ def lora_merge(d, W, sign, stream) -> None:
 def convert(src, src_dtype, dst, dst_dtype, n, stream) -> None:
     """mft_convert: bf16 -> fp32 (exact) or fp32 -> bf16 (the reference's RNE) on the device."""
     check(lib().mft_convert(src, int(src_dtype), dst, int(dst_dtype), int(n), stream))
+
+
+def layer_norm_desc(N, D, dtype=MFT_F32, eps=1e-5, x_stride=0, y_stride=0, dy_stride=0, dx_stride=0):
+    """Row strides in elements (0 = D)."""
+    return LayerNormDesc(N, D, dtype, eps, x_stride, y_stride, dy_stride, dx_stride)
+
+
+def layer_norm_fwd(d, x, weight, bias, y, mean, rstd, stream) -> None:
+    check(lib().mft_layer_norm_fwd(C.byref(d), x, weight, bias, y, mean, rstd, stream))
+
+
+def layer_norm_workspace_size(d) -> int:
+    n = C.c_size_t()
+    check(lib().mft_layer_norm_workspace_size(C.byref(d), C.byref(n)))
+    return n.value
+
+
+def layer_norm_bwd(d, x, weight, mean, rstd, dy, dx, dweight, dbias, workspace, stream) -> None:
+    check(lib().mft_layer_norm_bwd(C.byref(d), x, weight, mean, rstd, dy, dx, dweight, dbias, workspace, stream))
+
+
+def linear_desc(N, in_dim, out_dim, dtype=MFT_F32, w_transposed=False, activation=MFT_ACT_NONE):
+    return LinearDesc(N, in_dim, out_dim, dtype, int(bool(w_transposed)), activation)
+
+
+def linear_workspace_size(d):
+    f, b = C.c_size_t(), C.c_size_t()
+    check(lib().mft_linear_workspace_size(C.byref(d), C.byref(f), C.byref(b)))
+    return f.value, b.value
+
+
+def linear_fwd(d, x, W, bias, residual, y, z, workspace, stream) -> None:
+    check(lib().mft_linear_fwd(C.byref(d), x, W, bias, residual, y, z, workspace, stream))
+
+
+def linear_bwd(d, x, W, z, dy, dx, dW, dbias, workspace, stream) -> None:
+    check(lib().mft_linear_bwd(C.byref(d), x, W, z, dy, dx, dW, dbias, workspace, stream))
+
+
+def logprobs_desc(N, V, ld=0, grad_ld=0, dtype=MFT_F32, ignore_index=-100, top=0):
+    return LogprobsDesc(N, V, ld, grad_ld, dtype, ignore_index, top)
+
+
+def logprobs_workspace_size(d) -> int:
+    n = C.c_size_t()
+    check(lib().mft_logprobs_workspace_size(C.byref(d), C.byref(n)))
+    return n.value
+
+
+def logprobs_fwd(d, logits, tokens, logprob, entropy, stats, top_logprobs, top_ids, status, workspace, stream) -> None:
+    check(lib().mft_logprobs_fwd(C.byref(d), logits, tokens, logprob, entropy, stats, top_logprobs, top_ids, status,
+                                 workspace, stream))
+
+
+def logprobs_bwd(d, logits, tokens, stats, entropy, grad_logprob, grad_entropy, grad_logits, stream) -> None:
+    check(lib().mft_logprobs_bwd(C.byref(d), logits, tokens, stats, entropy, grad_logprob, grad_entropy, grad_logits,
+                                 stream))

@@ -1,0 +1,424 @@
+// Layer norm over the last dimension, forward and backward (C ABI in
+// include/mft/layer_norm.h).
+//
+// A row is held in registers, by one wave (WPR = 1), four or sixteen: one read
+// of x, the mean, then the sums of d = x - mean and d^2 about it, so that a
+// mean far above the deviation costs no digits (the sum of d, which is zero but
+// for the mean's rounding, corrects the mean by the part it was rounded by).
+// Longer rows are read once per sum.  All of it is bound by memory.
+//
+// Backward: the row sums of g = dy w and g h give dx in one pass over x and dy.
+// The sums over rows, dw and db, stay in registers: a workgroup takes rows
+// g, g + groups, ... and leaves one partial [2][D], and a second launch adds
+// the partials in their order, so results do not depend on the schedule.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "attn_kernels.h"
+#include "layer_norm_kernels.h"
+#include "row_util.h"
+
+namespace mft {
+namespace {
+
+template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
+
+// Sums of two values over the WPR waves of a row, in every thread.  `s` is
+// scratch of 2 * WPR floats that no other call in flight uses.
+template <int WPR> __device__ __forceinline__ void row_sum2(float& a, float& b, float* s) {
+    a = wave_sum_f(a);
+    b = wave_sum_f(b);
+    if constexpr (WPR > 1) {
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+            s[2 * w] = a;
+            s[2 * w + 1] = b;
+        }
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int i = 0; i < WPR; ++i) {
+            a += s[2 * i];
+            b += s[2 * i + 1];
+        }
+    }
+}
+
+template <int WPR> constexpr int kThreads = WPR == 1 ? 256 : 64 * WPR;
+
+template <typename T, int WPR, int CH>
+__global__ __launch_bounds__(kThreads<WPR>) void ln_fwd(LayerNormArgs a) {
+    constexpr int V = kVec<T>, TPR = 64 * WPR;
+    __shared__ float s1[2 * WPR], s2[2 * WPR];
+    const int t = threadIdx.x % TPR;
+    const int64_t n = (int64_t)blockIdx.x * (kThreads<WPR> / TPR) + threadIdx.x / TPR;
+    if (n >= a.N) return;  // whole waves: a workgroup of one row has n < N
+    const T* xr = (const T*)a.x + n * a.sx;
+    float x[CH][V];
+    float sum = 0.f, none = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) load_part<T, V>(xr, (int64_t)(c * TPR + t) * V, a.D, x[c]);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum += x[c][e];
+    row_sum2<WPR>(sum, none, s1);
+    const float inv = 1.0f / (float)a.D;
+    float mean = sum * inv, d1 = 0.f, d2 = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float d = (int64_t)(c * TPR + t) * V + e < a.D ? x[c][e] - mean : 0.f;
+            x[c][e] = d;
+            d1 += d;
+            d2 = fmaf(d, d, d2);
+        }
+    row_sum2<WPR>(d1, d2, s2);
+    const float off = d1 * inv;  // what the mean's rounding left
+    const float rstd = 1.0f / sqrtf(fmaxf(fmaf(-off, off, d2 * inv), 0.f) + a.eps);
+    T* yr = (T*)a.y + n * a.sy;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int64_t d0 = (int64_t)(c * TPR + t) * V;
+        if (d0 >= a.D) break;
+        float w[V], b[V];
+        if (a.w) load_part<float, V>(a.w, d0, a.D, w);
+        if (a.b) load_part<float, V>(a.b, d0, a.D, b);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float h = (x[c][e] - off) * rstd;
+            x[c][e] = a.w ? (a.b ? fmaf(h, w[e], b[e]) : h * w[e]) : (a.b ? h + b[e] : h);
+        }
+        store_part<T, V>(yr, d0, a.D, x[c]);
+    }
+    if (t == 0) {
+        if (a.mean) a.mean[n] = mean + off;
+        if (a.rstd) a.rstd[n] = rstd;
+    }
+}
+
+// Rows too long for registers: one workgroup reads the row once per sum and
+// once to write.
+constexpr int kLongThreads = 1024, kLongWaves = 16;
+template <typename T> __global__ __launch_bounds__(kLongThreads) void ln_fwd_long(LayerNormArgs a) {
+    constexpr int V = kVec<T>;
+    __shared__ float s1[2 * kLongWaves], s2[2 * kLongWaves];
+    const int64_t n = blockIdx.x;
+    const T* xr = (const T*)a.x + n * a.sx;
+    const float inv = 1.0f / (float)a.D;
+    float sum = 0.f, none = 0.f;
+    for (int64_t d0 = (int64_t)threadIdx.x * V; d0 < a.D; d0 += kLongThreads * V) {
+        float x[V], p = 0.f;
+        load_part<T, V>(xr, d0, a.D, x);
+#pragma unroll
+        for (int e = 0; e < V; ++e) p += x[e];
+        sum += p;
+    }
+    row_sum2<kLongWaves>(sum, none, s1);
+    const float mean = sum * inv;
+    float d1 = 0.f, d2 = 0.f;
+    for (int64_t d0 = (int64_t)threadIdx.x * V; d0 < a.D; d0 += kLongThreads * V) {
+        float x[V], p1 = 0.f, p2 = 0.f;
+        load_part<T, V>(xr, d0, a.D, x);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float d = d0 + e < a.D ? x[e] - mean : 0.f;
+            p1 += d;
+            p2 = fmaf(d, d, p2);
+        }
+        d1 += p1;
+        d2 += p2;
+    }
+    row_sum2<kLongWaves>(d1, d2, s2);
+    const float off = d1 * inv;
+    const float rstd = 1.0f / sqrtf(fmaxf(fmaf(-off, off, d2 * inv), 0.f) + a.eps);
+    T* yr = (T*)a.y + n * a.sy;
+    for (int64_t d0 = (int64_t)threadIdx.x * V; d0 < a.D; d0 += kLongThreads * V) {
+        float x[V], w[V], b[V];
+        load_part<T, V>(xr, d0, a.D, x);
+        if (a.w) load_part<float, V>(a.w, d0, a.D, w);
+        if (a.b) load_part<float, V>(a.b, d0, a.D, b);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float h = ((x[e] - mean) - off) * rstd;
+            x[e] = a.w ? (a.b ? fmaf(h, w[e], b[e]) : h * w[e]) : (a.b ? h + b[e] : h);
+        }
+        store_part<T, V>(yr, d0, a.D, x);
+    }
+    if (threadIdx.x == 0) {
+        if (a.mean) a.mean[n] = mean + off;
+        if (a.rstd) a.rstd[n] = rstd;
+    }
+}
+
+// Workgroup g: rows in steps of groups * (rows a workgroup holds at once).
+template <typename T, int WPR, int CH, bool PARAMS>
+__global__ __launch_bounds__(kThreads<WPR>) void ln_bwd(LayerNormArgs a) {
+    constexpr int V = kVec<T>, TPR = 64 * WPR, RPB = kThreads<WPR> / TPR;
+    extern __shared__ float lds[];  // PARAMS and RPB > 1: [2][D]
+    __shared__ float s[2][2 * WPR];
+    const int t = threadIdx.x % TPR;
+    const float inv = 1.0f / (float)a.D;
+    float dw[CH][V], db[CH][V], w[CH][V];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int64_t d0 = (int64_t)(c * TPR + t) * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) dw[c][e] = db[c][e] = 0.f, w[c][e] = 1.f;
+        if (a.w) load_part<float, V>(a.w, d0, a.D, w[c]);
+    }
+    int turn = 0;
+    for (int64_t n = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; n < a.N; n += a.groups * RPB) {
+        const T* xr = (const T*)a.x + n * a.sx;
+        const T* gr = (const T*)a.dy + n * a.sdy;
+        float h[CH][V], g[CH][V];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int64_t d0 = (int64_t)(c * TPR + t) * V;
+            load_part<T, V>(xr, d0, a.D, h[c]);
+            load_part<T, V>(gr, d0, a.D, g[c]);  // 0 past the end, and with it all below
+        }
+        const float mean = a.mean_in[n], rstd = a.rstd_in[n];
+        float c1 = 0.f, c2 = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                h[c][e] = (h[c][e] - mean) * rstd;
+                if constexpr (PARAMS) {
+                    dw[c][e] = fmaf(g[c][e], h[c][e], dw[c][e]);
+                    db[c][e] += g[c][e];
+                }
+                g[c][e] *= w[c][e];
+                c1 += g[c][e];
+                c2 = fmaf(g[c][e], h[c][e], c2);
+            }
+        if (a.dx) {
+            row_sum2<WPR>(c1, c2, s[turn]);
+            turn ^= 1;
+            c1 *= inv;
+            c2 *= inv;
+            T* dr = (T*)a.dx + n * a.sdx;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int64_t d0 = (int64_t)(c * TPR + t) * V;
+                if (d0 >= a.D) break;
+#pragma unroll
+                for (int e = 0; e < V; ++e) g[c][e] = rstd * (g[c][e] - c1 - h[c][e] * c2);
+                store_part<T, V>(dr, d0, a.D, g[c]);
+            }
+        }
+    }
+    if constexpr (PARAMS) {
+        float* out = a.part + (int64_t)blockIdx.x * 2 * a.D;
+        if constexpr (RPB > 1) {  // the waves add in turn
+            for (int i = 0; i < RPB; ++i) {
+                if (threadIdx.x / TPR == i)
+#pragma unroll
+                    for (int c = 0; c < CH; ++c)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            const int64_t d = (int64_t)(c * TPR + t) * V + e;
+                            if (d < a.D) {
+                                lds[d] = dw[c][e] + (i ? lds[d] : 0.f);
+                                lds[a.D + d] = db[c][e] + (i ? lds[a.D + d] : 0.f);
+                            }
+                        }
+                __syncthreads();
+            }
+            for (int64_t d = threadIdx.x; d < 2 * a.D; d += kThreads<WPR>) out[d] = lds[d];
+        } else {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int64_t d0 = (int64_t)(c * TPR + t) * V;
+                store_part<float, V>(out, d0, a.D, dw[c]);
+                store_part<float, V>(out + a.D, d0, a.D, db[c]);
+            }
+        }
+    }
+}
+
+// Rows too long for registers: their two sums, then dx and the partials of dw
+// and db by columns.
+template <typename T> __global__ __launch_bounds__(kLongThreads) void ln_bwd_sums(LayerNormArgs a) {
+    constexpr int V = kVec<T>;
+    __shared__ float s[2 * kLongWaves];
+    const int64_t n = blockIdx.x;
+    const T* xr = (const T*)a.x + n * a.sx;
+    const T* gr = (const T*)a.dy + n * a.sdy;
+    const float mean = a.mean_in[n], rstd = a.rstd_in[n];
+    float c1 = 0.f, c2 = 0.f;
+    for (int64_t d0 = (int64_t)threadIdx.x * V; d0 < a.D; d0 += kLongThreads * V) {
+        float x[V], g[V], w[V], p1 = 0.f, p2 = 0.f;
+        load_part<T, V>(xr, d0, a.D, x);
+        load_part<T, V>(gr, d0, a.D, g);
+        if (a.w) load_part<float, V>(a.w, d0, a.D, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float q = a.w ? g[e] * w[e] : g[e];
+            p1 += q;
+            p2 = fmaf(q, (x[e] - mean) * rstd, p2);
+        }
+        c1 += p1;
+        c2 += p2;
+    }
+    row_sum2<kLongWaves>(c1, c2, s);
+    if (threadIdx.x == 0) a.sums[n] = make_float2(c1, c2);
+}
+
+template <typename T> __global__ __launch_bounds__(256) void ln_bwd_columns(LayerNormArgs a) {
+    const int64_t d = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (d >= a.D) return;
+    const float inv = 1.0f / (float)a.D, w = a.w ? a.w[d] : 1.f;
+    float dw = 0.f, db = 0.f;
+#pragma unroll 4
+    for (int64_t n = blockIdx.y; n < a.N; n += a.groups) {
+        const float rstd = a.rstd_in[n], h = ((float)((const T*)a.x)[n * a.sx + d] - a.mean_in[n]) * rstd;
+        const float g = (float)((const T*)a.dy)[n * a.sdy + d];
+        dw = fmaf(g, h, dw);
+        db += g;
+        if (a.dx) {
+            const float2 c = a.sums[n];
+            ((T*)a.dx)[n * a.sdx + d] = (T)(rstd * (g * w - c.x * inv - h * (c.y * inv)));
+        }
+    }
+    if (a.part) {
+        float* out = a.part + (int64_t)blockIdx.y * 2 * a.D;
+        out[d] = dw;
+        out[a.D + d] = db;
+    }
+}
+
+// dw and db: the groups' partials in order.  64 columns to a workgroup; its 16
+// waves take the groups in turn.
+__global__ __launch_bounds__(1024) void ln_params(LayerNormArgs a) {
+    __shared__ float s[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane, C = 2 * a.D;
+    float v = 0.f;
+    if (c < C)
+#pragma unroll 8
+        for (int64_t g = w; g < a.groups; g += 16) v += a.part[g * C + c];
+    s[w][lane] = v;
+    __syncthreads();
+    if (w != 0 || c >= C) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) v += s[i][lane];
+    if (c < a.D) {
+        if (a.dw) a.dw[c] = v;
+    } else if (a.db) {
+        a.db[c - a.D] = v;
+    }
+}
+
+__global__ __launch_bounds__(256) void ln_zero_params(LayerNormArgs a) {
+    const int64_t d = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (d >= a.D) return;
+    if (a.dw) a.dw[d] = 0.f;
+    if (a.db) a.db[d] = 0.f;
+}
+
+// Waves to a row and 16-byte chunks to a thread.  WPR 0: by memory.
+struct Shape {
+    int wpr, ch;
+};
+Shape fwd_shape(int64_t D, int vec) {
+    for (const Shape s : {Shape{1, 1}, {1, 2}, {1, 4}, {1, 8}, {4, 4}, {4, 8}, {16, 4}, {16, 8}})
+        if (D <= (int64_t)64 * s.wpr * s.ch * vec) return s;
+    return {0, 0};
+}
+Shape bwd_shape(int64_t D, int vec) {
+    for (const Shape s : {Shape{1, 1}, {1, 2}, {1, 4}, {4, 2}, {4, 4}, {16, 2}})
+        if (D <= (int64_t)64 * s.wpr * s.ch * vec) return s;
+    return {0, 0};
+}
+int64_t bwd_groups(int64_t N, int64_t D, int vec) {
+    const Shape s = bwd_shape(D, vec);
+    const int64_t at_once = s.wpr == 1 ? 4 : 1, most = s.wpr == 16 || s.wpr == 0 ? 1 : 2;
+    return std::max<int64_t>(1, std::min<int64_t>((N + at_once - 1) / at_once, most * device_cus()));
+}
+size_t up(size_t x) { return (x + 255) & ~size_t(255); }
+
+template <typename T> hipError_t fwd(const LayerNormArgs& a, hipStream_t st) {
+    const Shape s = fwd_shape(a.D, kVec<T>);
+    const dim3 grid((unsigned)(s.wpr == 1 ? (a.N + 3) / 4 : a.N));
+#define MFT_LN_FWD(WPR, CH) \
+    if (s.wpr == WPR && s.ch == CH) hipLaunchKernelGGL((ln_fwd<T, WPR, CH>), grid, dim3(kThreads<WPR>), 0, st, a)
+    MFT_LN_FWD(1, 1);
+    MFT_LN_FWD(1, 2);
+    MFT_LN_FWD(1, 4);
+    MFT_LN_FWD(1, 8);
+    MFT_LN_FWD(4, 4);
+    MFT_LN_FWD(4, 8);
+    MFT_LN_FWD(16, 4);
+    MFT_LN_FWD(16, 8);
+#undef MFT_LN_FWD
+    if (s.wpr == 0) hipLaunchKernelGGL((ln_fwd_long<T>), grid, dim3(kLongThreads), 0, st, a);
+    return hipGetLastError();
+}
+
+template <typename T> hipError_t bwd(const LayerNormArgs& a, hipStream_t st) {
+    const Shape s = bwd_shape(a.D, kVec<T>);
+    const bool params = a.dw || a.db;
+    if (s.wpr == 0) {
+        LayerNormArgs q = a;
+        if (!params) q.part = nullptr;
+        if (a.dx) {
+            hipLaunchKernelGGL((ln_bwd_sums<T>), dim3((unsigned)a.N), dim3(kLongThreads), 0, st, q);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+        hipLaunchKernelGGL((ln_bwd_columns<T>), dim3((unsigned)((a.D + 255) / 256), (unsigned)a.groups), dim3(256), 0,
+                           st, q);
+    }
+#define MFT_LN_BWD(WPR, CH)                                                                                     \
+    if (s.wpr == WPR && s.ch == CH) {                                                                           \
+        const size_t lds = params && WPR == 1 ? (size_t)a.D * 8 : 0;                                            \
+        const dim3 grid((unsigned)a.groups), block(kThreads<WPR>);                                              \
+        if (params) hipLaunchKernelGGL((ln_bwd<T, WPR, CH, true>), grid, block, (unsigned)lds, st, a);          \
+        else hipLaunchKernelGGL((ln_bwd<T, WPR, CH, false>), grid, block, 0, st, a);                            \
+    }
+    MFT_LN_BWD(1, 1)
+    MFT_LN_BWD(1, 2)
+    MFT_LN_BWD(1, 4)
+    MFT_LN_BWD(4, 2)
+    MFT_LN_BWD(4, 4)
+    MFT_LN_BWD(16, 2)
+#undef MFT_LN_BWD
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !params) return e;
+    hipLaunchKernelGGL(ln_params, dim3((unsigned)((2 * a.D + 63) / 64)), dim3(1024), 0, st, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_layer_norm_fwd(const LayerNormArgs& a, bool is_bf16, hipStream_t st) {
+    if (a.N == 0) return hipSuccess;
+    return is_bf16 ? fwd<bf16>(a, st) : fwd<float>(a, st);
+}
+
+size_t layer_norm_workspace(int64_t N, int64_t D, bool is_bf16) {
+    const int vec = is_bf16 ? kVec<bf16> : kVec<float>;
+    size_t n = up((size_t)bwd_groups(N, D, vec) * 2 * D * 4);
+    if (bwd_shape(D, vec).wpr == 0) n += up((size_t)N * sizeof(float2));
+    return n;
+}
+
+hipError_t launch_layer_norm_bwd(LayerNormArgs a, bool is_bf16, void* workspace, hipStream_t st) {
+    if (a.N == 0) {
+        if (!a.dw && !a.db) return hipSuccess;
+        hipLaunchKernelGGL(ln_zero_params, dim3((unsigned)((a.D + 255) / 256)), dim3(256), 0, st, a);
+        return hipGetLastError();
+    }
+    if (!a.dx && !a.dw && !a.db) return hipSuccess;
+    const int vec = is_bf16 ? kVec<bf16> : kVec<float>;
+    a.groups = bwd_groups(a.N, a.D, vec);
+    a.part = static_cast<float*>(workspace);
+    a.sums = reinterpret_cast<float2*>(static_cast<char*>(workspace) + up((size_t)a.groups * 2 * a.D * 4));
+    return is_bf16 ? bwd<bf16>(a, st) : bwd<float>(a, st);
+}
+
+}  // namespace mft

@@ -1,0 +1,41 @@
+// Launchers of the linear layer's kernels (linear_gemm.hip, linear.hip; called
+// by linear_capi.cpp).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace mft {
+
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU_TANH = 2, ACT_SILU = 3 };
+
+// C[M, N] = act(sum_k P(m, k) Q(n, k) + bias[n]) + residual, all bf16 but bias.
+// P is stored [M, K] (p_kc) or [K, M], Q [N, K] (q_kc) or [K, N], contiguous.
+struct BfGemm {
+    int64_t M, N, K;
+    const void* P;
+    const void* Q;
+    int p_kc, q_kc;
+    void* C;
+    // epilogue
+    const float* bias;     // [N] or null
+    const void* residual;  // [M, N] or null
+    void* z;               // [M, N], before the activation, or null
+    int act;
+    float* partial;        // workspace of bf_gemm_workspace bytes
+};
+size_t bf_gemm_workspace(const BfGemm& g);
+hipError_t launch_bf_gemm(const BfGemm& g, hipStream_t st);
+
+// y = act(z) + residual over n values; y may be z or residual.
+hipError_t launch_act(const float* z, const float* residual, float* y, int64_t n, int act, hipStream_t st);
+
+// dz = dy act'(z) ([N, out]; no act: dz is not written) and db[out] = the sums
+// of dz's columns before rounding (null: left out).
+size_t dz_workspace(int64_t N, int64_t out);
+hipError_t launch_dz(const void* dy, const void* z, void* dz, float* db, int64_t N, int64_t out, int act, bool bf16,
+                     float* workspace, hipStream_t st);
+hipError_t launch_fill_zero(void* p, size_t bytes, hipStream_t st);  // bytes: a multiple of 2
+
+}  // namespace mft

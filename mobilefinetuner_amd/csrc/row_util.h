@@ -1,0 +1,73 @@
+// Device helpers of the row-wise passes: loads and stores of a few consecutive
+// elements at any element address, and sums over a wave in registers.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "attn_common.h"
+
+namespace mft {
+
+// V consecutive elements of type T as floats.  The vector type has T's
+// alignment: a wide access may start at any element (rows of odd length).
+template <typename T, int V> struct AnyVec {
+    typedef T raw __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+    __device__ __forceinline__ static raw load_raw(const T* p) { return *reinterpret_cast<const raw*>(p); }
+    __device__ __forceinline__ static void load(const T* p, float* x) {
+        const raw r = load_raw(p);
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] = (float)r[e];
+    }
+    __device__ __forceinline__ static void store(T* p, const float* x) {
+        raw r;
+#pragma unroll
+        for (int e = 0; e < V; ++e) r[e] = (T)x[e];
+        *reinterpret_cast<raw*>(p) = r;
+    }
+};
+
+// Elements d0 .. d0 + V - 1 of a row of D elements, zero past its end.
+template <typename T, int V>
+__device__ __forceinline__ void load_part(const T* row, int64_t d0, int64_t D, float* x) {
+    if (d0 + V <= D) {
+        AnyVec<T, V>::load(row + d0, x);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] = d0 + e < D ? (float)row[d0 + e] : 0.f;
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_part(T* row, int64_t d0, int64_t D, const float* x) {
+    if (d0 + V <= D) {
+        AnyVec<T, V>::store(row + d0, x);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (d0 + e < D) row[d0 + e] = (T)x[e];
+    }
+}
+
+template <int CTRL> __device__ __forceinline__ float dpp(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+// Sum over the wave, the same bits in every lane: pairs by DPP within rows of
+// 16 lanes (quads by permutation, then mirrored halves and rows), then by lane
+// swaps across them.  All lanes must be active.
+__device__ __forceinline__ float wave_sum_f(float x) {
+    x += dpp<0xB1>(x);   // quad_perm [1, 0, 3, 2]
+    x += dpp<0x4E>(x);   // quad_perm [2, 3, 0, 1]
+    x += dpp<0x141>(x);  // row_half_mirror
+    x += dpp<0x140>(x);  // row_mirror
+    x = row16_sum(x);
+    return half_sum(x);
+}
+__device__ __forceinline__ float wave_max_f(float x) {
+    x = fmaxf(x, dpp<0xB1>(x));
+    x = fmaxf(x, dpp<0x4E>(x));
+    x = fmaxf(x, dpp<0x141>(x));
+    x = fmaxf(x, dpp<0x140>(x));
+    x = row16_max(x);
+    return half_max(x);
+}
+
+}  // namespace mft

@@ -1,0 +1,69 @@
+"""What the torch helpers share: checks of operands, the device and stream a
+call is enqueued on, and workspaces.
+
+A call runs on the device of its first operand, whichever is current, and on
+torch's current stream of that device.  Outputs and workspaces are torch
+tensors allocated under that stream, so the caching allocator hands their
+memory out again only in its order.
+"""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import capi
+
+DTYPES = {torch.float32: capi.MFT_F32, torch.bfloat16: capi.MFT_BF16}
+_HERE = contextlib.nullcontext()
+
+
+def guard(t):
+    """Makes t's device current for a `with` block."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def operand(t, name, like=None, dtype=None, shape=None):
+    """t, checked: on the GPU (`like`'s, if given), of `dtype` and `shape` where they are given."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor (there is no CPU path)")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, the call on {like.device}")
+    if dtype is None:
+        if t.dtype not in DTYPES:
+            raise ValueError(f"{name}: unsupported dtype {t.dtype}")
+    elif t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    return t
+
+
+def optional(t, name, like, dtype, shape):
+    """A contiguous operand that may be None."""
+    return None if t is None else operand(t, name, like, dtype, shape).contiguous()
+
+
+def rows(t, last):
+    """t [..., last] as [N, last] with one stride between rows: a view where its
+    strides allow, else a copy."""
+    if t.dim() != 2:
+        t = t.reshape(-1, last)
+    if t.stride(1) == 1 or last == 1:
+        if t.stride(0) >= last:
+            return t
+        if t.shape[0] <= 1:
+            return t.as_strided(t.shape, (last, 1))
+    return t.contiguous()
+
+
+def workspace(nbytes, like):
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
