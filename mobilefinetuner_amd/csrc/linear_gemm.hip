@@ -3,19 +3,32 @@
 //
 // A workgroup of 2 x 2 waves owns a BN x BM tile of C^T = Q P^T, on
 // v_mfma_f32_32x32x16_bf16: Q's rows are the instruction's rows, so that a lane
-// holds four consecutive columns n of one row m of C.  Either operand is stored
-// with k contiguous (a tile is [rows][BK], fragments are 16-byte reads) or with
-// its rows contiguous (a tile is [BK][rows], fragments are transposing reads).
-// A stage of BK values of k comes by direct loads into LDS where all rows and
-// bases lie on 16 bytes (DMA), the stage after next while one is multiplied;
-// else, and for the last stage where BK does not divide K, through registers
-// with zeros past the end.
+// holds four consecutive columns n of one row m of C.
+//
+// Operands.  With k contiguous (KC) an operand lies in LDS as slabs [rows][64]
+// and its fragments are 16-byte reads; a slab's rows are whole 128-byte lines
+// (slabs of 32 took every line from L2 twice: 25 M requests for 13 M at 4096^3,
+// and 157 us for 124).  With its rows contiguous it lies as slabs [32][rows] and
+// its fragments are transposing reads.  Either way by direct loads into LDS
+// where all rows and bases lie on 16 bytes (DMA), else through registers.
+//
+// Pipeline (DMA), in halves of 32 k: two slabs of 64 or three of 32 are in LDS.
+// A wave reads the fragments of a half's second step while it multiplies the
+// first; then one barrier tells that everybody has read the half and that the
+// next has landed, the loads of the half three on go out into the freed slabs,
+// and the next half's first fragments are read while the second step
+// multiplies.  Two workgroups share a CU: one multiplies while the other waits
+// or runs its epilogue.
+//
+// Epilogue.  The accumulators go through LDS, 32 rows of m at a time and wave by
+// wave, so that y, z and the residual move in whole lines.
 //
 // Products of few tiles cut K into slices whose fp32 partials a second launch
 // adds in their order and takes through the epilogue.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_common.h"
 #include "attn_geometry.h"
@@ -30,53 +43,60 @@ namespace {
 
 constexpr int kThreads = 256;
 
+constexpr int kHalf = 32, kSlab = 64;  // k of a pipeline step, and of a slab with k contiguous
+
 struct Args {
     BfGemm g;
-    int tiles_m, tiles_n, slices, stages, per_slice;
-    int whole;  // one slice: the epilogue in the product's launch
+    int tiles_m, tiles_n, slices;
+    int halves, per_slice;  // whole halves that go in pairs; of one slice (even)
+    int whole;              // one slice: the epilogue in the product's launch
     FastDiv per_slice_tiles;
 };
 
-// 16-byte chunk c of row r in a tile with k contiguous: 16 rows' reads of one
-// chunk meet no bank twice.
-template <int BK> __device__ __forceinline__ constexpr int swz_kc(int r) {
-    return BK == 32 ? (r >> 2) & 3 : (r >> 1) & 7;
-}
+__device__ __forceinline__ constexpr int swz_kc(int r) { return (r >> 1) & 7; }  // 16 rows' reads of a chunk: 16 banks' groups
 
-// One operand of R rows a tile: its loads and its fragments.
-template <int R, int BK, bool KC> struct Operand {
-    static constexpr int kBytes = R * BK * 2, PER = kBytes / 1024 / 4;  // 1 KiB loads of a wave
-    static constexpr int ROW = KC ? BK : R, CPR = ROW / 8, RPL = 64 / CPR;  // LDS row, chunks of it, rows of a load
-    static_assert(PER >= 1 && PER * 4096 == kBytes && RPL >= 1, "whole loads");
-    // Tile row (KC: the operand's row, else k) and chunk of this lane's load j.
-    __device__ __forceinline__ static int load_row(int w, int j, int lane) { return (w * PER + j) * RPL + lane / CPR; }
-    __device__ __forceinline__ static int load_chunk(int row, int lane) {
-        const int p = lane % CPR;
-        return KC ? p ^ swz_kc<BK>(row) : p ^ swz_tr<CPR>(row);
+// One operand of R rows a tile.
+template <int R, bool KC> struct Operand {
+    static constexpr int kSlabBytes = KC ? R * kSlab * 2 : R * kHalf * 2, kRing = KC ? 2 : 3;
+    static constexpr int kBytes = kRing * kSlabBytes;
+    static constexpr int ROW = KC ? kSlab : R, CPR = ROW / 8;  // elements and chunks of an LDS row
+    static constexpr int PER = kSlabBytes / 4096;              // direct loads (1 KiB) of a wave per slab
+    static constexpr int HALF = R / 64;                        // 16-byte chunks of a thread per half
+    // The slab that holds half h (an offset in the operand's LDS).
+    __device__ __forceinline__ static int slab(int h) {
+        return KC ? (h >> 1 & 1) * kSlabBytes : (int)((unsigned)h % 3u) * kSlabBytes;
     }
-    // Direct loads: this lane's byte offsets from the tile's first element.
-    uint32_t off[PER];
-    __device__ __forceinline__ void init(int w, int lane, int64_t r0, int64_t rows, int64_t ld) {
+    __device__ __forceinline__ static int swz_of(int r) { return KC ? swz_kc(r) : swz_tr<CPR>(r); }
+
+    // Direct loads: this lane's byte offsets from a slab's first element.
+    struct Dma {
+        uint32_t off[PER];
+        __device__ __forceinline__ void init(int w, int lane, int64_t r0, int64_t rows, int64_t ld) {
+            static_assert(PER * 4096 == kSlabBytes && 64 % CPR == 0, "whole loads of whole rows");
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int r = load_row(w, j, lane), c = load_chunk(r, lane);
-            if (KC)  // rows past the end are read again from the last one, and not stored
-                off[j] = (uint32_t)((min(r0 + r, rows - 1) - r0) * ld * 2) + 16u * c;
-            else
-                off[j] = (uint32_t)(r * ld * 2) + (uint32_t)(min(r0 + 8 * c, rows - 8) - r0) * 2u;
+            for (int j = 0; j < PER; ++j) {
+                const int r = (w * PER + j) * (64 / CPR) + lane / CPR, c = lane % CPR ^ swz_of(r);
+                if (KC)  // rows past the end are read again from the last one, and not stored
+                    off[j] = (uint32_t)((min(r0 + r, rows - 1) - r0) * ld * 2) + 16u * c;
+                else
+                    off[j] = (uint32_t)(r * ld * 2) + (uint32_t)(min(r0 + 8 * c, rows - 8) - r0) * 2u;
+            }
         }
-    }
-    __device__ __forceinline__ void issue(const char* tile, uint32_t lds, int w) const {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) load_lds_16_s(tile, off[j], lds + (uint32_t)(w * PER + j) * 1024u);
-    }
-    // The same loads through registers, anywhere and with zeros past the ends.
+        // Load j of the slab whose first element is `from`, into the slab at LDS address `to`.
+        __device__ __forceinline__ void issue(const char* from, uint32_t to, int w, int j) const {
+            load_lds_16_s(from, off[j], to + (uint32_t)(w * PER + j) * 1024u);
+        }
+    };
+
+    // A half through registers, from anywhere and with zeros past the ends.
     typedef bf16 any8 __attribute__((ext_vector_type(8), aligned(2)));
+    __device__ __forceinline__ static int half_row(int j, int tid) { return KC ? (j * kThreads + tid) / 4 : (j * kThreads + tid) / CPR; }
+    __device__ __forceinline__ static int half_chunk(int j, int tid) { return KC ? tid % 4 : (j * kThreads + tid) % CPR; }
     __device__ __forceinline__ static bf16x8 fetch(const bf16* p, int64_t ld, int64_t r0, int64_t rows, int64_t k0,
-                                                   int64_t K, int w, int j, int lane) {
-        const int r = load_row(w, j, lane), c = load_chunk(r, lane);
-        const int64_t row = KC ? min(r0 + r, rows - 1) : k0 + r;       // storage row
-        const int64_t col = KC ? k0 + 8 * c : r0 + 8 * c, end = KC ? K : rows;
+                                                   int64_t K, int j, int tid) {
+        const int r = half_row(j, tid), c = half_chunk(j, tid);
+        const int64_t row = KC ? min(r0 + r, rows - 1) : k0 + r;  // storage row
+        const int64_t col = (KC ? k0 : r0) + 8 * c, end = KC ? K : rows;
         bf16x8 v = zero_vec<bf16x8>();
         if (!KC && row >= K) return v;
         const bf16* q = p + row * ld + col;
@@ -89,20 +109,21 @@ template <int R, int BK, bool KC> struct Operand {
         }
         return v;
     }
-    __device__ __forceinline__ static void store(char* lds, int w, int j, int lane, bf16x8 v) {
-        *reinterpret_cast<bf16x8*>(lds + (w * PER + j) * 1024 + lane * 16) = v;
+    __device__ __forceinline__ static void store(char* lds, int h, int j, int tid, bf16x8 v) {  // h even
+        const int r = half_row(j, tid), c = half_chunk(j, tid);
+        *reinterpret_cast<bf16x8*>(lds + slab(h) + r * ROW * 2 + (c ^ swz_of(r)) * 16) = v;
     }
 };
 
-// Fragments of T 32-row tiles from row `first` on, k step ks of a stage.
-template <int R, int BK, bool KC, int T> struct Fragments {
-    uint32_t at[KC ? BK / 16 : T];
+// Fragments of T 32-row tiles from row `first` on.
+template <int R, bool KC, int T> struct Fragments {
+    uint32_t at[KC ? kSlab / 16 : T];
     __device__ __forceinline__ void init(int first, int lane) {
         const int n = lane & 31, hh = lane >> 5;
         if constexpr (KC) {
 #pragma unroll
-            for (int ks = 0; ks < BK / 16; ++ks)
-                at[ks] = (uint32_t)((first + n) * BK * 2 + ((2 * ks + hh) ^ swz_kc<BK>(n)) * 16);
+            for (int i = 0; i < kSlab / 16; ++i)
+                at[i] = (uint32_t)((first + n) * kSlab * 2 + ((2 * i + hh) ^ swz_kc(n)) * 16);
         } else {
             const int j = lane & 15, k = 8 * hh + j / 4;
 #pragma unroll
@@ -112,9 +133,10 @@ template <int R, int BK, bool KC, int T> struct Fragments {
             }
         }
     }
-    __device__ __forceinline__ bf16x8 read(const char* lds, int ks, int t) const {
+    // Tile t, step ks (0, 1) of a half, the second of its pair if `odd`, in the slab at `lds`.
+    __device__ __forceinline__ bf16x8 read(const char* lds, bool odd, int ks, int t) const {
         if constexpr (KC) {
-            return *reinterpret_cast<const bf16x8*>(lds + at[ks] + t * 32 * BK * 2);
+            return *reinterpret_cast<const bf16x8*>(lds + at[2 * odd + ks] + t * 32 * kSlab * 2);
         } else {
             const char* p = lds + at[t] + ks * 16 * R * 2;
             const bf16x4 a = ds_read_tr4(reinterpret_cast<const bf16*>(p));
@@ -146,13 +168,15 @@ __device__ __forceinline__ void epilogue(const BfGemm& g, int64_t m, int64_t n, 
     store_part<bf16, V>((bf16*)g.C + m * g.N, n, g.N, v);
 }
 
-template <int BN, int BM, int BK, bool PKC, bool QKC, bool DMA, int ACT>
+template <int BN, int BM, bool PKC, bool QKC, bool DMA, int ACT>
 __global__ __launch_bounds__(kThreads, 2) void bf_gemm_kernel(Args a) {
     constexpr int TN = BN / 64, TM = BM / 64;  // 32 x 32 tiles of a wave
-    typedef Operand<BM, BK, PKC> OpP;
-    typedef Operand<BN, BK, QKC> OpQ;
-    constexpr int kStage = OpP::kBytes + OpQ::kBytes, kBufs = DMA ? 3 : 2;
-    __shared__ __attribute__((aligned(1024))) char smem[kBufs * kStage];  // [buffer][Q, P]
+    typedef Operand<BM, PKC> OpP;
+    typedef Operand<BN, QKC> OpQ;
+    constexpr int WN = BN / 2, kPitch = WN + 4;  // the epilogue's rows of fp32, a bank group apart
+    constexpr int kStaged = 4 * 32 * kPitch * 4, kSlabs = OpQ::kBytes + OpP::kBytes;
+    __shared__ __attribute__((aligned(1024))) char smem[kSlabs > kStaged ? kSlabs : kStaged];  // [Q slabs][P slabs]
+    char* const lds_p = smem + OpQ::kBytes;
     const int lane = threadIdx.x & 63, w = wave_id(), hh = lane >> 5;
     const int wn = w & 1, wm = w >> 1;
 
@@ -166,12 +190,14 @@ __global__ __launch_bounds__(kThreads, 2) void bf_gemm_kernel(Args a) {
     // scalars, whatever unit divides: the direct loads take their bases from them
     const int tn = __builtin_amdgcn_readfirstlane(col), tm = __builtin_amdgcn_readfirstlane(band * kBand + in - col * high);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-    const int s0 = slice * a.per_slice, s1 = min(s0 + a.per_slice, a.stages);
+    const bool last = slice == a.slices - 1;
+    // Halves of this slice, and where the last one's k end (the rest of K goes through registers).
+    const int h0 = slice * a.per_slice, h1 = last ? a.halves : h0 + a.per_slice;
 
     const int64_t ldp = PKC ? a.g.K : a.g.M, ldq = QKC ? a.g.K : a.g.N;
     const bf16 *P = (const bf16*)a.g.P, *Q = (const bf16*)a.g.Q;
-    Fragments<BM, BK, PKC, TM> fp;
-    Fragments<BN, BK, QKC, TN> fq;
+    Fragments<BM, PKC, TM> fp;
+    Fragments<BN, QKC, TN> fq;
     fp.init(wm * BM / 2, lane);
     fq.init(wn * BN / 2, lane);
     f32x16 acc[TN][TM];
@@ -182,109 +208,177 @@ __global__ __launch_bounds__(kThreads, 2) void bf_gemm_kernel(Args a) {
             acc[j][k] = zero16();
             asm volatile("" : "+v"(acc[j][k]));  // not a literal zero (see mfma_v_first)
         }
-    auto multiply = [&](const char* q, const char* p) {
-        struct Ops {
-            bf16x8 q[TN], p[TM];
-        };
-        auto read = [&](int ks) {
-            Ops o;
-#pragma unroll
-            for (int t = 0; t < TN; ++t) o.q[t] = fq.read(q, ks, t);
-#pragma unroll
-            for (int t = 0; t < TM; ++t) o.p[t] = fp.read(p, ks, t);
-            return o;
-        };
-        Ops cur = read(0);
-#pragma unroll
-        for (int ks = 0; ks < BK / 16; ++ks) {
-            Ops next;
-            if (ks + 1 < BK / 16) next = read(ks + 1);
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int k = 0; k < TM; ++k) acc[j][k] = mfma_bf16(cur.q[j], cur.p[k], acc[j][k]);
-            if (ks + 1 < BK / 16) cur = next;
-        }
-        pin_read_ahead<BK / 16, 1, Fragments<BM, BK, PKC, TM>::kReads + Fragments<BN, BK, QKC, TN>::kReads, TN * TM>();
+    struct Ops {
+        bf16x8 q[TN], p[TM];
     };
-    bf16x8 rp[OpP::PER], rq[OpQ::PER];
-    auto fetch = [&](int s) {
-        const int64_t k0 = (int64_t)s * BK;
+    auto read = [&](int h, bool odd, int ks) {
+        Ops o;
+        const char *q = smem + OpQ::slab(h), *p = lds_p + OpP::slab(h);
 #pragma unroll
-        for (int j = 0; j < OpQ::PER; ++j) rq[j] = OpQ::fetch(Q, ldq, n0, a.g.N, k0, a.g.K, w, j, lane);
+        for (int t = 0; t < TN; ++t) o.q[t] = fq.read(q, odd, ks, t);
 #pragma unroll
-        for (int j = 0; j < OpP::PER; ++j) rp[j] = OpP::fetch(P, ldp, m0, a.g.M, k0, a.g.K, w, j, lane);
+        for (int t = 0; t < TM; ++t) o.p[t] = fp.read(p, odd, ks, t);
+        return o;
     };
-    auto store = [&](char* stage) {
+    constexpr int kTiles = TN * TM;
+    auto multiply = [&](const Ops& o, int t0 = 0, int t1 = 1 << 10) {
 #pragma unroll
-        for (int j = 0; j < OpQ::PER; ++j) OpQ::store(stage, w, j, lane, rq[j]);
-#pragma unroll
-        for (int j = 0; j < OpP::PER; ++j) OpP::store(stage + OpQ::kBytes, w, j, lane, rp[j]);
+        for (int t = 0; t < kTiles; ++t)
+            if (t >= t0 && t < t1) acc[t / TM][t % TM] = mfma_bf16(o.q[t / TM], o.p[t % TM], acc[t / TM][t % TM]);
     };
+    constexpr int kReads = Fragments<BM, PKC, TM>::kReads + Fragments<BN, QKC, TN>::kReads;
 
     if constexpr (DMA) {
-        OpP op;
-        OpQ oq;
-        op.init(w, lane, m0, a.g.M, ldp);
-        oq.init(w, lane, n0, a.g.N, ldq);
-        const char* tp = reinterpret_cast<const char*>(P + (PKC ? m0 * ldp : m0));
-        const char* tq = reinterpret_cast<const char*>(Q + (QKC ? n0 * ldq : n0));
-        const int64_t step_p = (int64_t)BK * 2 * (PKC ? 1 : ldp), step_q = (int64_t)BK * 2 * (QKC ? 1 : ldq);
-        const uint32_t base = lds_addr(smem);
-        auto issue = [&](int s, int buf) {
-            oq.issue(tq + s * step_q, base + (uint32_t)(buf * kStage), w);
-            op.issue(tp + s * step_p, base + (uint32_t)(buf * kStage + OpQ::kBytes), w);
+        if (h0 < h1) {
+            typename OpP::Dma dp;
+            typename OpQ::Dma dq;
+            dp.init(w, lane, m0, a.g.M, ldp);
+            dq.init(w, lane, n0, a.g.N, ldq);
+            const char* tp = reinterpret_cast<const char*>(P + (PKC ? m0 * ldp : m0));
+            const char* tq = reinterpret_cast<const char*>(Q + (QKC ? n0 * ldq : n0));
+            const int64_t step_p = (int64_t)kHalf * 2 * (PKC ? 1 : ldp), step_q = (int64_t)kHalf * 2 * (QKC ? 1 : ldq);
+            const uint32_t base = lds_addr(smem);
+            // The loads of half h, ODD its place in its pair (a slab of 64 comes with its even half).
+            auto issue = [&](int h, auto odd_t) {
+                constexpr bool ODD = decltype(odd_t)::value;
+                if constexpr (!(QKC && ODD)) {
+                    const char* from = tq + h * step_q;
+                    const uint32_t to = base + (uint32_t)OpQ::slab(h);
+#pragma unroll
+                    for (int j = 0; j < OpQ::PER; ++j) dq.issue(from, to, w, j);
+                }
+                if constexpr (!(PKC && ODD)) {
+                    const char* from = tp + h * step_p;
+                    const uint32_t to = base + (uint32_t)(OpQ::kBytes + OpP::slab(h));
+#pragma unroll
+                    for (int j = 0; j < OpP::PER; ++j) dp.issue(from, to, w, j);
+                }
+            };
+            constexpr std::false_type even{};
+            constexpr std::true_type odd{};
+            constexpr int kEven = OpQ::PER + OpP::PER, kOdd = (QKC ? 0 : OpQ::PER) + (PKC ? 0 : OpP::PER);
+            issue(h0, even);
+            issue(h0 + 1, odd);
+            if (h0 + 2 < h1) {
+                issue(h0 + 2, even);
+                wait_vmcnt<kEven + kOdd>();
+            } else {
+                wait_vmcnt<kOdd>();
+            }
+            lds_barrier();
+            Ops cur = read(h0, false, 0);
+            // N MFMAs with R LDS reads between them, in this order.
+            auto spread = [](auto n_t, auto r_t) {
+                constexpr int N = decltype(n_t)::value, R = decltype(r_t)::value, E = (R + N - 1) / N;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
+                    if (i * E < R) __builtin_amdgcn_sched_group_barrier(SG_DS_READ, E, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            // One half, ODD its place in its pair; LEFT: halves after it (3: at least three).
+            auto half = [&](int h, auto odd_t, auto left_t) {
+                constexpr bool ODD = decltype(odd_t)::value;
+                constexpr int LEFT = decltype(left_t)::value;
+                const Ops nxt = read(h, ODD, 1);
+                multiply(cur);
+                spread(std::integral_constant<int, kTiles>{}, std::integral_constant<int, kReads>{});
+                if constexpr (LEFT >= 1) {
+                    // Half h + 1 has landed (h + 2 may be on its way), and all of half h is read.
+                    wait_vmcnt<LEFT == 1 ? 0 : ODD ? kOdd : kEven>();
+                    lds_barrier();
+                    constexpr int kFirst = (kTiles + 1) / 2;
+                    cur = read(h + 1, !ODD, 0);
+                    multiply(nxt, 0, kFirst);
+                    spread(std::integral_constant<int, kFirst>{}, std::integral_constant<int, kReads>{});
+                    if constexpr (LEFT >= 3) issue(h + 3, std::bool_constant<!ODD>{});
+                    __builtin_amdgcn_sched_barrier(0);
+                    multiply(nxt, kFirst);
+                    __builtin_amdgcn_sched_barrier(0);
+                } else {
+                    multiply(nxt);
+                }
+            };
+            constexpr std::integral_constant<int, 0> left0{};
+            constexpr std::integral_constant<int, 1> left1{};
+            constexpr std::integral_constant<int, 2> left2{};
+            constexpr std::integral_constant<int, 3> left3{};
+            int h = h0;
+            for (; h + 4 < h1; h += 2) {
+                half(h, even, left3);
+                half(h + 1, odd, left3);
+            }
+            if (h + 2 < h1) {
+                half(h, even, left3);
+                half(h + 1, odd, left2);
+                h += 2;
+            }
+            half(h, even, left1);
+            half(h + 1, odd, left0);
+        }
+    }
+    // What is left of K in pairs of halves, or all of it, half by half through registers.
+    const int from = DMA ? a.halves : h0, to = DMA || last ? (int)((a.g.K + kHalf - 1) / kHalf) : h1;
+    if (!DMA || last) {
+        bf16x8 rp[OpP::HALF], rq[OpQ::HALF];
+        auto fetch = [&](int h) {
+            const int64_t k0 = (int64_t)h * kHalf;
+#pragma unroll
+            for (int j = 0; j < OpQ::HALF; ++j) rq[j] = OpQ::fetch(Q, ldq, n0, a.g.N, k0, a.g.K, j, threadIdx.x);
+#pragma unroll
+            for (int j = 0; j < OpP::HALF; ++j) rp[j] = OpP::fetch(P, ldp, m0, a.g.M, k0, a.g.K, j, threadIdx.x);
         };
-        const int sf = min(s1, (int)(a.g.K / BK));  // whole stages
-        if (s0 < sf) issue(s0, 0);
-        if (s0 + 1 < sf) issue(s0 + 1, 1);
-        int buf = 0;
-        for (int s = s0; s < sf; ++s) {
-            // Stage s has landed in every wave's share, and every wave is done
-            // with stage s - 1, whose buffer stage s + 2 takes.
-            if (s + 1 < sf) wait_vmcnt<OpP::PER + OpQ::PER>();
-            else wait_vmcnt<0>();
-            lds_barrier();
-            if (s + 2 < sf) issue(s + 2, buf == 0 ? 2 : buf - 1);
-            multiply(smem + buf * kStage, smem + buf * kStage + OpQ::kBytes);
-            buf = buf == 2 ? 0 : buf + 1;
+        if (from < to) {
+            fetch(from);
+            if (DMA) lds_barrier();  // everybody has read the last pair
         }
-        if (sf < s1) {  // the last, partial stage
-            fetch(sf);
+        for (int h = from; h < to; ++h) {
+            // Two are in LDS at a time, each the even half of its slab: a wave stores one once all
+            // have read the one before the last.
+            const int i = 2 * (h - from);
+#pragma unroll
+            for (int j = 0; j < OpQ::HALF; ++j) OpQ::store(smem, i, j, threadIdx.x, rq[j]);
+#pragma unroll
+            for (int j = 0; j < OpP::HALF; ++j) OpP::store(lds_p, i, j, threadIdx.x, rp[j]);
             lds_barrier();
-            store(smem);
-            lds_barrier();
-            multiply(smem, smem + OpQ::kBytes);
-        }
-    } else {
-        fetch(s0);
-        store(smem);
-        lds_barrier();
-        int buf = 0;
-        for (int s = s0; s < s1; ++s) {
-            if (s + 1 < s1) fetch(s + 1);
-            multiply(smem + buf * kStage, smem + buf * kStage + OpQ::kBytes);
-            buf ^= 1;
-            if (s + 1 < s1) store(smem + buf * kStage);
-            lds_barrier();
+            if (h + 1 < to) fetch(h + 1);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) multiply(read(i, false, ks));
         }
     }
 
-    const int64_t mw = m0 + wm * (BM / 2) + (lane & 31), nw = n0 + wn * (BN / 2) + 4 * hh;
+    // The accumulators, 32 rows of m at a time, through this wave's part of LDS.
+    lds_barrier();
+    float* st = reinterpret_cast<float*>(smem) + w * 32 * kPitch;
+    constexpr int V = 8, LPR = WN / V;  // lanes to a row
+    const int64_t nw = n0 + wn * WN;
 #pragma unroll
     for (int k = 0; k < TM; ++k) {
-        const int64_t m = mw + 32 * k;
-        if (m >= a.g.M) continue;
+        const int64_t mw = m0 + wm * (BM / 2) + 32 * k;
+        if (mw >= a.g.M) break;
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int64_t n = nw + 32 * j + 8 * q;
-                if (n >= a.g.N) continue;
-                float v[4] = {acc[j][k][4 * q], acc[j][k][4 * q + 1], acc[j][k][4 * q + 2], acc[j][k][4 * q + 3]};
-                if (a.whole) epilogue<ACT, 4>(a.g, m, n, v);
-                else store_part<float, 4>(a.g.partial + ((int64_t)slice * a.g.M + m) * a.g.N, n, a.g.N, v);
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<f32x4*>(st + (lane & 31) * kPitch + 32 * j + 8 * q + 4 * hh) =
+                    f32x4{acc[j][k][4 * q], acc[j][k][4 * q + 1], acc[j][k][4 * q + 2], acc[j][k][4 * q + 3]};
+        asm volatile("" ::: "memory");  // a wave's LDS accesses stay in order
+#pragma unroll
+        for (int r = 0; r < LPR / 2; ++r) {
+            const int at = r * 64 + lane, row = at / LPR, c = at % LPR * V;
+            const int64_t m = mw + row, n = nw + c;
+            if (m >= a.g.M || n >= a.g.N) continue;
+            float v[V];
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                const f32x4 u = *reinterpret_cast<const f32x4*>(st + row * kPitch + c + e);
+                v[e] = u[0], v[e + 1] = u[1], v[e + 2] = u[2], v[e + 3] = u[3];
             }
+            if (a.whole) epilogue<ACT, V>(a.g, m, n, v);
+            else store_part<float, V>(a.g.partial + ((int64_t)slice * a.g.M + m) * a.g.N, n, a.g.N, v);
+        }
+        asm volatile("" ::: "memory");
     }
 }
 
@@ -308,16 +402,18 @@ template <int ACT> __global__ __launch_bounds__(256) void bf_gemm_reduce(Args a)
 bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 struct Plan {
-    int shape;  // 0: 256 x 128 (n x m), 1: 128 x 128, 2: 64 x 64
+    int shape;
     Args a;
 };
-constexpr int kBN[3] = {256, 128, 64}, kBM[3] = {128, 128, 64}, kBK[3] = {32, 32, 64};
+constexpr int kShapes = 3;
+constexpr int kBN[kShapes] = {256, 128, 64}, kBM[kShapes] = {128, 128, 64};
 
 Plan plan(const BfGemm& g) {
     Plan p{};
     const int cus = device_cus();
     auto tiles = [&](int s) { return ((g.N + kBN[s] - 1) / kBN[s]) * ((g.M + kBM[s] - 1) / kBM[s]); };
     p.shape = tiles(0) >= cus ? 0 : tiles(1) >= cus ? 1 : 2;
+    if (p.shape == 0 && g.p_kc && g.q_kc) p.shape = 1;
     int64_t slices = 1;
     if (p.shape == 2) {
         if (tiles(1) * (g.K / 512) >= cus) p.shape = 1;
@@ -328,24 +424,33 @@ Plan plan(const BfGemm& g) {
     p.a.g = g;
     p.a.tiles_m = (int)((g.M + kBM[s] - 1) / kBM[s]);
     p.a.tiles_n = (int)((g.N + kBN[s] - 1) / kBN[s]);
-    p.a.stages = (int)((g.K + kBK[s] - 1) / kBK[s]);
-    p.a.per_slice = (int)((p.a.stages + slices - 1) / slices);
-    p.a.slices = (p.a.stages + p.a.per_slice - 1) / p.a.per_slice;
+    const int pairs = (int)(g.K / kSlab);
+    p.a.halves = 2 * pairs;
+    const int per = std::max<int>(1, (int)((pairs + slices - 1) / slices));
+    p.a.per_slice = 2 * per;
+    p.a.slices = std::max(1, (pairs + per - 1) / per);
     p.a.whole = p.a.slices == 1;
     p.a.per_slice_tiles = FastDiv::make((uint32_t)(p.a.tiles_m * p.a.tiles_n));
     return p;
 }
 
-template <int BN, int BM, int BK, bool PKC, bool QKC, int ACT>
-void launch_t(const Args& a, bool dma, hipStream_t st) {
+template <int BN, int BM, bool PKC, bool QKC, int ACT> void launch_t(const Args& a, bool dma, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.tiles_m * a.tiles_n * a.slices));
-    if (dma) hipLaunchKernelGGL((bf_gemm_kernel<BN, BM, BK, PKC, QKC, true, ACT>), grid, dim3(kThreads), 0, st, a);
-    else hipLaunchKernelGGL((bf_gemm_kernel<BN, BM, BK, PKC, QKC, false, ACT>), grid, dim3(kThreads), 0, st, a);
+    if (dma) hipLaunchKernelGGL((bf_gemm_kernel<BN, BM, PKC, QKC, true, ACT>), grid, dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL((bf_gemm_kernel<BN, BM, PKC, QKC, false, ACT>), grid, dim3(kThreads), 0, st, a);
 }
 template <bool PKC, bool QKC, int ACT> void launch_s(const Plan& p, bool dma, hipStream_t st) {
-    if (p.shape == 0) launch_t<256, 128, 32, PKC, QKC, ACT>(p.a, dma, st);
-    else if (p.shape == 1) launch_t<128, 128, 32, PKC, QKC, ACT>(p.a, dma, st);
-    else launch_t<64, 64, 64, PKC, QKC, ACT>(p.a, dma, st);
+    if (p.shape == 2) {
+        launch_t<64, 64, PKC, QKC, ACT>(p.a, dma, st);
+        return;
+    }
+    if constexpr (!(PKC && QKC)) {
+        if (p.shape == 0) {
+            launch_t<256, 128, PKC, QKC, ACT>(p.a, dma, st);
+            return;
+        }
+    }
+    launch_t<128, 128, PKC, QKC, ACT>(p.a, dma, st);
 }
 template <int ACT> void launch_act_fwd(const Plan& p, bool dma, hipStream_t st) {
     if (p.a.g.q_kc) launch_s<true, true, ACT>(p, dma, st);
