@@ -28,6 +28,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "attn_common.h"
@@ -169,7 +170,7 @@ __device__ __forceinline__ void epilogue(const BfGemm& g, int64_t m, int64_t n, 
 }
 
 template <int BN, int BM, bool PKC, bool QKC, bool DMA, int ACT>
-__global__ __launch_bounds__(kThreads, 2) void bf_gemm_kernel(Args a) {
+__global__ __launch_bounds__(kThreads, BN * BM > 32768 ? 1 : 2) void bf_gemm_kernel(Args a) {
     constexpr int TN = BN / 64, TM = BM / 64;  // 32 x 32 tiles of a wave
     typedef Operand<BM, PKC> OpP;
     typedef Operand<BN, QKC> OpQ;
@@ -206,27 +207,32 @@ __global__ __launch_bounds__(kThreads, 2) void bf_gemm_kernel(Args a) {
 #pragma unroll
         for (int k = 0; k < TM; ++k) {
             acc[j][k] = zero16();
-            asm volatile("" : "+v"(acc[j][k]));  // not a literal zero (see mfma_v_first)
+            // not a literal zero (see mfma_v_first)
+            if constexpr (TN * TM > 8) asm volatile("" : "+a"(acc[j][k]));
+            else asm volatile("" : "+v"(acc[j][k]));
         }
     struct Ops {
         bf16x8 q[TN], p[TM];
     };
+    constexpr int kTiles = TN * TM, kFrags = TN + TM;
+    // Fragment f of step ks of half h (the second of its pair if `odd`).
+    auto read_one = [&](Ops& o, int h, bool odd, int ks, int f) {
+        if (f < TM) o.p[f] = fp.read(lds_p + OpP::slab(h), odd, ks, f);
+        else o.q[f - TM] = fq.read(smem + OpQ::slab(h), odd, ks, f - TM);
+    };
     auto read = [&](int h, bool odd, int ks) {
         Ops o;
-        const char *q = smem + OpQ::slab(h), *p = lds_p + OpP::slab(h);
 #pragma unroll
-        for (int t = 0; t < TN; ++t) o.q[t] = fq.read(q, odd, ks, t);
-#pragma unroll
-        for (int t = 0; t < TM; ++t) o.p[t] = fp.read(p, odd, ks, t);
+        for (int f = 0; f < kFrags; ++f) read_one(o, h, odd, ks, f);
         return o;
     };
-    constexpr int kTiles = TN * TM;
-    auto multiply = [&](const Ops& o, int t0 = 0, int t1 = 1 << 10) {
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-            if (t >= t0 && t < t1) acc[t / TM][t % TM] = mfma_bf16(o.q[t / TM], o.p[t % TM], acc[t / TM][t % TM]);
+    auto multiply_one = [&](const Ops& o, int t) {
+        acc[t / TM][t % TM] = mfma_bf16(o.q[t / TM], o.p[t % TM], acc[t / TM][t % TM]);
     };
-    constexpr int kReads = Fragments<BM, PKC, TM>::kReads + Fragments<BN, QKC, TN>::kReads;
+    auto multiply = [&](const Ops& o) {
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) multiply_one(o, t);
+    };
 
     if constexpr (DMA) {
         if (h0 < h1) {
@@ -238,68 +244,73 @@ __global__ __launch_bounds__(kThreads, 2) void bf_gemm_kernel(Args a) {
             const char* tq = reinterpret_cast<const char*>(Q + (QKC ? n0 * ldq : n0));
             const int64_t step_p = (int64_t)kHalf * 2 * (PKC ? 1 : ldp), step_q = (int64_t)kHalf * 2 * (QKC ? 1 : ldq);
             const uint32_t base = lds_addr(smem);
-            // The loads of half h, ODD its place in its pair (a slab of 64 comes with its even half).
-            auto issue = [&](int h, auto odd_t) {
+            // Load j of half h, ODD its place in its pair (a slab of 64 comes with its even half).
+            auto issue_one = [&](int h, auto odd_t, int j) {
                 constexpr bool ODD = decltype(odd_t)::value;
-                if constexpr (!(QKC && ODD)) {
-                    const char* from = tq + h * step_q;
-                    const uint32_t to = base + (uint32_t)OpQ::slab(h);
-#pragma unroll
-                    for (int j = 0; j < OpQ::PER; ++j) dq.issue(from, to, w, j);
-                }
-                if constexpr (!(PKC && ODD)) {
-                    const char* from = tp + h * step_p;
-                    const uint32_t to = base + (uint32_t)(OpQ::kBytes + OpP::slab(h));
-#pragma unroll
-                    for (int j = 0; j < OpP::PER; ++j) dp.issue(from, to, w, j);
-                }
+                constexpr int NQ = QKC && ODD ? 0 : OpQ::PER;
+                if (j < NQ) dq.issue(tq + h * step_q, base + (uint32_t)OpQ::slab(h), w, j);
+                else dp.issue(tp + h * step_p, base + (uint32_t)(OpQ::kBytes + OpP::slab(h)), w, j - NQ);
             };
             constexpr std::false_type even{};
             constexpr std::true_type odd{};
             constexpr int kEven = OpQ::PER + OpP::PER, kOdd = (QKC ? 0 : OpQ::PER) + (PKC ? 0 : OpP::PER);
+            auto issue = [&](int h, auto odd_t) {
+#pragma unroll
+                for (int j = 0; j < (decltype(odd_t)::value ? kOdd : kEven); ++j) issue_one(h, odd_t, j);
+            };
             issue(h0, even);
             issue(h0 + 1, odd);
-            if (h0 + 2 < h1) {
-                issue(h0 + 2, even);
-                wait_vmcnt<kEven + kOdd>();
-            } else {
-                wait_vmcnt<kOdd>();
-            }
+            wait_vmcnt<kOdd>();
             lds_barrier();
             Ops cur = read(h0, false, 0);
-            // N MFMAs with R LDS reads between them, in this order.
-            auto spread = [](auto n_t, auto r_t) {
-                constexpr int N = decltype(n_t)::value, R = decltype(r_t)::value, E = (R + N - 1) / N;
+            // A step's MFMAs, with the next step's fragment reads and a share of the loads of a
+            // half between them: one after the other in this order, as a wave that issues many
+            // loads at once waits for them with nothing to multiply.
+            auto weave = [&](const Ops& o, auto&& reads, auto&& loads) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
-                    if (i * E < R) __builtin_amdgcn_sched_group_barrier(SG_DS_READ, E, 0);
+                for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+                    for (int f = t * kFrags / kTiles; f < (t + 1) * kFrags / kTiles; ++f) reads(f);
+                    multiply_one(o, t);
+                    loads(t);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             };
-            // One half, ODD its place in its pair; LEFT: halves after it (3: at least three).
+            // Share t of kTiles of a part (0: the first, 1: the second) of half h's loads.
+            auto share = [&](int h, auto odd_t, int part, int t) {
+                constexpr int n = decltype(odd_t)::value ? kOdd : kEven, first = (n + 1) / 2;
+                const int from = part ? first : 0, count = part ? n - first : first;
+#pragma unroll
+                for (int j = 0; j < n; ++j)
+                    if (j >= from + t * count / kTiles && j < from + (t + 1) * count / kTiles) issue_one(h, odd_t, j);
+            };
+            // One half, ODD its place in its pair; LEFT: halves after it (4: at least four).  The loads of
+            // half h + 3 go out behind the barrier, when half h's slabs are free, and in half h + 1.
             auto half = [&](int h, auto odd_t, auto left_t) {
                 constexpr bool ODD = decltype(odd_t)::value;
                 constexpr int LEFT = decltype(left_t)::value;
-                const Ops nxt = read(h, ODD, 1);
-                multiply(cur);
-                spread(std::integral_constant<int, kTiles>{}, std::integral_constant<int, kReads>{});
+                constexpr std::bool_constant<!ODD> other{};
+                Ops nxt;
+                weave(cur, [&](int f) { read_one(nxt, h, ODD, 1, f); },
+                      [&](int t) {
+                          if constexpr (LEFT >= 2) share(h + 2, odd_t, 1, t);
+                      });
                 if constexpr (LEFT >= 1) {
                     // Half h + 1 has landed (h + 2 may be on its way), and all of half h is read.
                     wait_vmcnt<LEFT == 1 ? 0 : ODD ? kOdd : kEven>();
                     lds_barrier();
-                    constexpr int kFirst = (kTiles + 1) / 2;
-                    cur = read(h + 1, !ODD, 0);
-                    multiply(nxt, 0, kFirst);
-                    spread(std::integral_constant<int, kFirst>{}, std::integral_constant<int, kReads>{});
-                    if constexpr (LEFT >= 3) issue(h + 3, std::bool_constant<!ODD>{});
-                    __builtin_amdgcn_sched_barrier(0);
-                    multiply(nxt, kFirst);
-                    __builtin_amdgcn_sched_barrier(0);
+                    weave(nxt, [&](int f) { read_one(cur, h + 1, !ODD, 0, f); },
+                          [&](int t) {
+                              if constexpr (LEFT >= 3) share(h + 3, other, 0, t);
+                          });
                 } else {
                     multiply(nxt);
                 }
             };
+            if (h0 + 2 < h1) {  // the first part of half h0 + 2, as if by the half before
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) share(h0 + 2, even, 0, t);
+            }
             constexpr std::integral_constant<int, 0> left0{};
             constexpr std::integral_constant<int, 1> left1{};
             constexpr std::integral_constant<int, 2> left2{};
@@ -405,28 +416,53 @@ struct Plan {
     int shape;
     Args a;
 };
-constexpr int kShapes = 3;
-constexpr int kBN[kShapes] = {256, 128, 64}, kBM[kShapes] = {128, 128, 64};
+
+// The tiles, and what each sustains over the whole GPU (TFLOP/s) with one
+// workgroup to a CU and with more, and the k that its prologue and epilogue are
+// worth (with an activation: `act` more).  Fitted to 42 products of 1 to 8192
+// rows and 640 to 6912 columns, each timed in every tile and cut into 1 to 16
+// slices: the choice by these is within 6 percent of the best, but for five, the
+// worst at 1.16 times it.  256 x 256 reads least of LDS and L2 per product, holds
+// its accumulators in all of a SIMD's registers and has nobody to overlap its
+// epilogue with (4096^3, W [out, in]: 112 us, 128 x 128 125; 8192 x 1024 -> 4096
+// with GELU 95, 256 x 128 86).  With k contiguous in both operands the slabs of
+// 256 x 128 do not leave a CU room for two.
+struct Shape {
+    int bn, bm;
+    double one, more;
+    int k, act;
+};
+constexpr Shape kShapes[] = {{256, 128, 1000, 1350, 330, 190},
+                             {128, 128, 900, 1080, 345, 190},
+                             {64, 64, 400, 760, 200, 100},
+                             {256, 256, 1400, 1400, 640, 200}};
+bool has_shape(const BfGemm& g, int s) { return s != 0 || (g.p_kc && !g.q_kc); }
 
 Plan plan(const BfGemm& g) {
     Plan p{};
-    const int cus = device_cus();
-    auto tiles = [&](int s) { return ((g.N + kBN[s] - 1) / kBN[s]) * ((g.M + kBM[s] - 1) / kBM[s]); };
-    p.shape = tiles(0) >= cus ? 0 : tiles(1) >= cus ? 1 : 2;
-    if (p.shape == 0 && g.p_kc && g.q_kc) p.shape = 1;
-    int64_t slices = 1;
-    if (p.shape == 2) {
-        if (tiles(1) * (g.K / 512) >= cus) p.shape = 1;
-        const int64_t t = tiles(p.shape);
-        if (2 * t < cus * 2) slices = std::max<int64_t>(1, std::min<int64_t>(2 * cus / t, g.K / 256));
+    const int cus = device_cus(), pairs = (int)(g.K / kSlab);
+    double best = 1e300;
+    int per = 1;
+    for (int s = 0; s < 4; ++s) {
+        if (!has_shape(g, s)) continue;
+        const Shape& t = kShapes[s];
+        const int64_t tiles = ((g.N + t.bn - 1) / t.bn) * ((g.M + t.bm - 1) / t.bm);
+        for (int slices : {1, 2, 3, 4, 6, 8, 12, 16}) {
+            if (slices > 1 && (slices > pairs || tiles * slices > 4 * cus)) break;
+            const int per_slice = std::max(1, (pairs + slices - 1) / slices), n = std::max(1, (pairs + per_slice - 1) / per_slice);
+            const double mean = (double)tiles * n / cus, most = std::ceil(mean);
+            const double rate = (most <= 1 ? t.one : t.more) * (g.p_kc && g.q_kc ? 1.1 : 1.0) * cus / 256;
+            double us = (most <= 1 ? 1 : (most + mean) / 2) * cus * t.bn * t.bm * 2 *
+                        ((double)g.K / n + t.k + (g.act != ACT_NONE && n == 1 ? t.act : 0)) / rate / 1e6;
+            if (n > 1) us += 5 + (double)n * g.M * g.N * 8 / 4.5e6;  // partials written and read, a launch
+            if (us < best * 0.999) best = us, p.shape = s, per = per_slice;
+        }
     }
-    const int s = p.shape;
+    const Shape& t = kShapes[p.shape];
     p.a.g = g;
-    p.a.tiles_m = (int)((g.M + kBM[s] - 1) / kBM[s]);
-    p.a.tiles_n = (int)((g.N + kBN[s] - 1) / kBN[s]);
-    const int pairs = (int)(g.K / kSlab);
+    p.a.tiles_m = (int)((g.M + t.bm - 1) / t.bm);
+    p.a.tiles_n = (int)((g.N + t.bn - 1) / t.bn);
     p.a.halves = 2 * pairs;
-    const int per = std::max<int>(1, (int)((pairs + slices - 1) / slices));
     p.a.per_slice = 2 * per;
     p.a.slices = std::max(1, (pairs + per - 1) / per);
     p.a.whole = p.a.slices == 1;
@@ -440,17 +476,12 @@ template <int BN, int BM, bool PKC, bool QKC, int ACT> void launch_t(const Args&
     else hipLaunchKernelGGL((bf_gemm_kernel<BN, BM, PKC, QKC, false, ACT>), grid, dim3(kThreads), 0, st, a);
 }
 template <bool PKC, bool QKC, int ACT> void launch_s(const Plan& p, bool dma, hipStream_t st) {
-    if (p.shape == 2) {
-        launch_t<64, 64, PKC, QKC, ACT>(p.a, dma, st);
-        return;
+    if constexpr (PKC && !QKC) {
+        if (p.shape == 0) launch_t<256, 128, PKC, QKC, ACT>(p.a, dma, st);
     }
-    if constexpr (!(PKC && QKC)) {
-        if (p.shape == 0) {
-            launch_t<256, 128, PKC, QKC, ACT>(p.a, dma, st);
-            return;
-        }
-    }
-    launch_t<128, 128, PKC, QKC, ACT>(p.a, dma, st);
+    if (p.shape == 1) launch_t<128, 128, PKC, QKC, ACT>(p.a, dma, st);
+    if (p.shape == 2) launch_t<64, 64, PKC, QKC, ACT>(p.a, dma, st);
+    if (p.shape == 3) launch_t<256, 256, PKC, QKC, ACT>(p.a, dma, st);
 }
 template <int ACT> void launch_act_fwd(const Plan& p, bool dma, hipStream_t st) {
     if (p.a.g.q_kc) launch_s<true, true, ACT>(p, dma, st);
