@@ -37,21 +37,21 @@ mft_status check(const mft_linear_desc* d, const char* who) {
 }
 
 // The three products.  fp32: terms[0] = (A, B) with the strides of the storage.
-mft::BfGemm bf_fwd(const mft_linear_desc* d) {
-    mft::BfGemm g{};
+mft::LinearProduct product_fwd(const mft_linear_desc* d) {
+    mft::LinearProduct g{};
     g.M = d->N, g.N = d->out_dim, g.K = d->in_dim;
     g.p_kc = 1, g.q_kc = d->w_transposed != 0;
     g.act = d->activation;
     return g;
 }
-mft::BfGemm bf_dx(const mft_linear_desc* d) {
-    mft::BfGemm g{};
+mft::LinearProduct product_dx(const mft_linear_desc* d) {
+    mft::LinearProduct g{};
     g.M = d->N, g.N = d->in_dim, g.K = d->out_dim;
     g.p_kc = 1, g.q_kc = d->w_transposed == 0;
     return g;
 }
-mft::BfGemm bf_dw(const mft_linear_desc* d) {  // rows: W's first dimension
-    mft::BfGemm g{};
+mft::LinearProduct product_dw(const mft_linear_desc* d) {  // rows: W's first dimension
+    mft::LinearProduct g{};
     g.M = d->w_transposed ? d->out_dim : d->in_dim;
     g.N = d->w_transposed ? d->in_dim : d->out_dim;
     g.K = d->N;
@@ -79,6 +79,10 @@ mft::GemmF32 f_dw(const mft_linear_desc* d) {
     return g;
 }
 
+size_t product_workspace(const mft::LinearProduct& g, const mft::GemmF32& f, bool bf) {
+    return mft::few_rows(g) ? 0 : bf ? mft::bf_gemm_workspace(g) : mft::gemm_f32_workspace(f);
+}
+
 struct BwdLayout {
     size_t dz, db, gemm, total;
 };
@@ -89,8 +93,7 @@ BwdLayout bwd_layout(const mft_linear_desc* d) {
     l.dz = o, o += d->activation == MFT_ACT_NONE ? 0 : up((size_t)d->N * d->out_dim * (bf ? 2 : 4));
     l.db = o, o += up(mft::dz_workspace(d->N, d->out_dim));
     l.gemm = o;
-    o += bf ? std::max(mft::bf_gemm_workspace(bf_dx(d)), mft::bf_gemm_workspace(bf_dw(d)))
-            : std::max(mft::gemm_f32_workspace(f_dx(d)), mft::gemm_f32_workspace(f_dw(d)));
+    o += std::max(product_workspace(product_dx(d), f_dx(d), bf), product_workspace(product_dw(d), f_dw(d), bf));
     l.total = o;
     return l;
 }
@@ -102,14 +105,14 @@ hipError_t run_f32(mft::GemmF32 g, const void* A, const void* B, void* C, char* 
     g.partial = reinterpret_cast<float*>(ws);
     return mft::launch_gemm_f32(g, st);
 }
-hipError_t run_bf(mft::BfGemm g, const void* P, const void* Q, void* C, char* ws, hipStream_t st) {
+// A bf16 product, or one of few rows of either type.
+hipError_t run(mft::LinearProduct g, bool bf, const void* P, const void* Q, void* C, char* ws, hipStream_t st) {
     g.P = P;
     g.Q = Q;
     g.C = C;
     g.partial = reinterpret_cast<float*>(ws);
-    return mft::launch_bf_gemm(g, st);
+    return mft::few_rows(g) ? mft::launch_few_rows(g, bf, st) : mft::launch_bf_gemm(g, st);
 }
-
 }  // namespace
 
 extern "C" {
@@ -119,9 +122,7 @@ mft_status mft_linear_workspace_size(const mft_linear_desc* desc, size_t* fwd_by
     if (r != MFT_OK) return r;
     const bool empty = desc->N == 0;
     if (fwd_bytes)
-        *fwd_bytes = empty ? 0
-                     : desc->dtype == MFT_BF16 ? mft::bf_gemm_workspace(bf_fwd(desc))
-                                               : mft::gemm_f32_workspace(f_fwd(desc));
+        *fwd_bytes = empty ? 0 : product_workspace(product_fwd(desc), f_fwd(desc), desc->dtype == MFT_BF16);
     if (bwd_bytes) *bwd_bytes = empty ? 0 : bwd_layout(desc).total;
     return MFT_OK;
 }
@@ -138,18 +139,17 @@ mft_status mft_linear_fwd(const mft_linear_desc* desc, const void* x, const void
     if (y == x || y == W || (z && (z == y || z == x || z == residual)))
         return fail(MFT_ERR_INVALID_ARG, "mft_linear_fwd: y may not be x or W, nor z another operand");
     char* ws = static_cast<char*>(workspace);
-    if (desc->dtype == MFT_BF16) {
-        mft::BfGemm g = bf_fwd(desc);
-        if (!ws && mft::bf_gemm_workspace(g) > 0)
-            return fail(MFT_ERR_INVALID_ARG, "mft_linear_fwd: workspace must be non-NULL");
-        g.bias = bias;
-        g.residual = residual;
-        g.z = z;
-        return hip_status(run_bf(g, x, W, y, ws, stream), "mft_linear_fwd launch");
+    const bool bf = desc->dtype == MFT_BF16;
+    mft::LinearProduct q = product_fwd(desc);
+    if (!ws && product_workspace(q, f_fwd(desc), bf) > 0)
+        return fail(MFT_ERR_INVALID_ARG, "mft_linear_fwd: workspace must be non-NULL");
+    if (bf || mft::few_rows(q)) {
+        q.bias = bias;
+        q.residual = residual;
+        q.z = z;
+        return hip_status(run(q, bf, x, W, y, ws, stream), "mft_linear_fwd launch");
     }
     mft::GemmF32 g = f_fwd(desc);
-    if (!ws && mft::gemm_f32_workspace(g) > 0)
-        return fail(MFT_ERR_INVALID_ARG, "mft_linear_fwd: workspace must be non-NULL");
     g.bias = bias;
     if (desc->activation == MFT_ACT_NONE) {
         if (residual == y) {
@@ -196,12 +196,12 @@ mft_status mft_linear_bwd(const mft_linear_desc* desc, const void* x, const void
     hipError_t e = mft::launch_dz(dy, z, dx || dW ? ws + l.dz : nullptr, dbias, desc->N, desc->out_dim,
                                   desc->activation, bf, reinterpret_cast<float*>(ws + l.db), stream);
     if (e == hipSuccess && dx)
-        e = bf ? run_bf(bf_dx(desc), dz, W, dx, ws + l.gemm, stream)
-               : run_f32(f_dx(desc), dz, W, dx, ws + l.gemm, stream);
+        e = bf || mft::few_rows(product_dx(desc)) ? run(product_dx(desc), bf, dz, W, dx, ws + l.gemm, stream)
+                                                  : run_f32(f_dx(desc), dz, W, dx, ws + l.gemm, stream);
     if (e == hipSuccess && dW) {
         const void* rows = desc->w_transposed ? dz : x;
         const void* cols = desc->w_transposed ? x : dz;
-        e = bf ? run_bf(bf_dw(desc), rows, cols, dW, ws + l.gemm, stream)
+        e = bf ? run(product_dw(desc), bf, rows, cols, dW, ws + l.gemm, stream)
                : run_f32(f_dw(desc), rows, cols, dW, ws + l.gemm, stream);
     }
     return hip_status(e, "mft_linear_bwd launch");

@@ -34,8 +34,7 @@
 #include "attn_common.h"
 #include "attn_geometry.h"
 #include "attn_kernels.h"
-#include "linear_act.h"
-#include "linear_kernels.h"
+#include "linear_epilogue.h"
 #include "prologue_kernels.h"
 #include "row_util.h"
 
@@ -47,7 +46,7 @@ constexpr int kThreads = 256;
 constexpr int kHalf = 32, kSlab = 64;  // k of a pipeline step, and of a slab with k contiguous
 
 struct Args {
-    BfGemm g;
+    LinearProduct g;
     int tiles_m, tiles_n, slices;
     int halves, per_slice;  // whole halves that go in pairs; of one slice (even)
     int whole;              // one slice: the epilogue in the product's launch
@@ -147,27 +146,6 @@ template <int R, bool KC, int T> struct Fragments {
     }
     static constexpr int kReads = KC ? T : 2 * T;
 };
-
-// y (and z) of V consecutive columns n of row m from their sums.
-template <int ACT, int V>
-__device__ __forceinline__ void epilogue(const BfGemm& g, int64_t m, int64_t n, float* v) {
-    if (g.bias) {
-        float b[V];
-        load_part<float, V>(g.bias, n, g.N, b);
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] += b[e];
-    }
-    if (ACT != ACT_NONE && g.z) store_part<bf16, V>((bf16*)g.z + m * g.N, n, g.N, v);
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = act_value<ACT>(v[e]);
-    if (g.residual) {
-        float r[V];
-        load_part<bf16, V>((const bf16*)g.residual + m * g.N, n, g.N, r);
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] += r[e];
-    }
-    store_part<bf16, V>((bf16*)g.C + m * g.N, n, g.N, v);
-}
 
 template <int BN, int BM, bool PKC, bool QKC, bool DMA, int ACT>
 __global__ __launch_bounds__(kThreads, BN * BM > 32768 ? 1 : 2) void bf_gemm_kernel(Args a) {
@@ -386,7 +364,7 @@ __global__ __launch_bounds__(kThreads, BN * BM > 32768 ? 1 : 2) void bf_gemm_ker
                 const f32x4 u = *reinterpret_cast<const f32x4*>(st + row * kPitch + c + e);
                 v[e] = u[0], v[e + 1] = u[1], v[e + 2] = u[2], v[e + 3] = u[3];
             }
-            if (a.whole) epilogue<ACT, V>(a.g, m, n, v);
+            if (a.whole) linear_epilogue<bf16, ACT, V>(a.g, m, n, v);
             else store_part<float, V>(a.g.partial + ((int64_t)slice * a.g.M + m) * a.g.N, n, a.g.N, v);
         }
         asm volatile("" ::: "memory");
@@ -407,7 +385,7 @@ template <int ACT> __global__ __launch_bounds__(256) void bf_gemm_reduce(Args a)
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] += p[e];
     }
-    epilogue<ACT, 4>(a.g, m, n, v);
+    linear_epilogue<bf16, ACT, 4>(a.g, m, n, v);
 }
 
 bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -436,9 +414,9 @@ constexpr Shape kShapes[] = {{256, 128, 1000, 1350, 330, 190},
                              {128, 128, 900, 1080, 345, 190},
                              {64, 64, 400, 760, 200, 100},
                              {256, 256, 1400, 1400, 640, 200}};
-bool has_shape(const BfGemm& g, int s) { return s != 0 || (g.p_kc && !g.q_kc); }
+bool has_shape(const LinearProduct& g, int s) { return s != 0 || (g.p_kc && !g.q_kc); }
 
-Plan plan(const BfGemm& g) {
+Plan plan(const LinearProduct& g) {
     Plan p{};
     const int cus = device_cus(), pairs = (int)(g.K / kSlab);
     double best = 1e300;
@@ -490,12 +468,12 @@ template <int ACT> void launch_act_fwd(const Plan& p, bool dma, hipStream_t st) 
 
 }  // namespace
 
-size_t bf_gemm_workspace(const BfGemm& g) {
+size_t bf_gemm_workspace(const LinearProduct& g) {
     const Plan p = plan(g);
     return p.a.whole ? 0 : (size_t)p.a.slices * g.M * g.N * 4;
 }
 
-hipError_t launch_bf_gemm(const BfGemm& g, hipStream_t st) {
+hipError_t launch_bf_gemm(const LinearProduct& g, hipStream_t st) {
     if (g.M <= 0 || g.N <= 0 || g.K <= 0) return hipSuccess;
     const Plan p = plan(g);
     const int64_t ldp = g.p_kc ? g.K : g.M, ldq = g.q_kc ? g.K : g.N;

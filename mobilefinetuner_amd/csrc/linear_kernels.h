@@ -1,5 +1,5 @@
-// Launchers of the linear layer's kernels (linear_gemm.hip, linear.hip; called
-// by linear_capi.cpp).
+// Launchers of the linear layer's kernels (linear_gemm.hip, linear_rows.hip,
+// linear.hip; called by linear_capi.cpp).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -10,9 +10,10 @@ namespace mft {
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU_TANH = 2, ACT_SILU = 3 };
 
-// C[M, N] = act(sum_k P(m, k) Q(n, k) + bias[n]) + residual, all bf16 but bias.
-// P is stored [M, K] (p_kc) or [K, M], Q [N, K] (q_kc) or [K, N], contiguous.
-struct BfGemm {
+// C[M, N] = act(sum_k P(m, k) Q(n, k) + bias[n]) + residual.  P is stored [M, K]
+// (p_kc) or [K, M], Q [N, K] (q_kc) or [K, N], all contiguous; all bf16, or all
+// fp32, but bias (fp32).
+struct LinearProduct {
     int64_t M, N, K;
     const void* P;
     const void* Q;
@@ -25,8 +26,12 @@ struct BfGemm {
     int act;
     float* partial;        // workspace of bf_gemm_workspace bytes
 };
-size_t bf_gemm_workspace(const BfGemm& g);
-hipError_t launch_bf_gemm(const BfGemm& g, hipStream_t st);
+// bf16, any sizes (linear_gemm.hip).
+size_t bf_gemm_workspace(const LinearProduct& g);
+hipError_t launch_bf_gemm(const LinearProduct& g, hipStream_t st);
+// Few rows with p_kc (linear_rows.hip); no workspace.
+bool few_rows(const LinearProduct& g);
+hipError_t launch_few_rows(const LinearProduct& g, bool bf16, hipStream_t st);
 
 // y = act(z) + residual over n values; y may be z or residual.
 hipError_t launch_act(const float* z, const float* residual, float* y, int64_t n, int act, hipStream_t st);

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import capi
-from .device import DTYPES, guard, operand, optional, ptr, rows, stream, workspace
+from .device import DTYPES, guard, like, operand, optional, ptr, rows, stream, workspace
 
 
 def _param(p, name, x):
@@ -26,9 +26,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     D, x2 = x.shape[-1], rows(x, x.shape[-1])
     w, b = _param(weight, "weight", x), _param(bias, "bias", x)
     with guard(x):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = like(x)
         mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
         d = capi.layer_norm_desc(x2.shape[0], D, DTYPES[x.dtype], eps, x2.stride(0))
         capi.layer_norm_fwd(d, x2.data_ptr(), ptr(w), ptr(b), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
                             stream(x))
@@ -46,9 +46,9 @@ def layer_norm_backward(x, weight, mean, rstd, dy, want_x=True, want_params=True
     mean = operand(mean, "mean", x, torch.float32, x.shape[:-1]).contiguous()
     rstd = operand(rstd, "rstd", x, torch.float32, x.shape[:-1]).contiguous()
     with guard(x):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
+        dx = like(x) if want_x else None
         dw = torch.empty(D, dtype=torch.float32, device=x.device) if want_params else None
-        db = torch.empty(D, dtype=torch.float32, device=x.device) if want_params else None
+        db = torch.empty_like(dw) if want_params else None
         d = capi.layer_norm_desc(x2.shape[0], D, DTYPES[x.dtype], 0.0, x2.stride(0), 0, g2.stride(0))
         ws = workspace(capi.layer_norm_workspace_size(d), x)
         capi.layer_norm_bwd(d, x2.data_ptr(), ptr(w), mean.data_ptr(), rstd.data_ptr(), g2.data_ptr(), ptr(dx),

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import capi
-from .device import DTYPES, guard, operand, ptr, stream, workspace
+from .device import DTYPES, guard, like, operand, ptr, stream, workspace
 
 ACTIVATIONS = {"none": capi.MFT_ACT_NONE, "relu": capi.MFT_ACT_RELU, "gelu_tanh": capi.MFT_ACT_GELU_TANH,
                "silu": capi.MFT_ACT_SILU}
@@ -69,8 +69,8 @@ def linear_backward(x, W, z, dy, activation="none", w_transposed=False, want_x=T
         z = None
     with guard(x):
         xc, Wc = x.contiguous(), W.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
-        dW = torch.empty(W.shape, dtype=W.dtype, device=x.device) if want_weight else None
+        dx = like(x) if want_x else None
+        dW = like(W) if want_weight else None
         db = torch.empty(n_out, dtype=torch.float32, device=x.device) if want_bias else None
         ws = workspace(capi.linear_workspace_size(d)[1], x)
         capi.linear_bwd(d, xc.data_ptr(), Wc.data_ptr(), ptr(z), dy.data_ptr(), ptr(dx), ptr(dW), ptr(db), ptr(ws),

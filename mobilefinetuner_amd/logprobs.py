@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import capi
-from .device import DTYPES, guard, operand, optional, ptr, rows, stream, workspace
+from .device import DTYPES, guard, like, operand, optional, ptr, rows, stream, workspace
 
 
 def _operands(logits, tokens):
@@ -33,10 +33,10 @@ def token_logprobs(logits, tokens, top=0, ignore_index=-100, check_tokens=True):
     with guard(logits):
         dev = logits.device
         logprob = torch.empty(lead, dtype=torch.float32, device=dev)
-        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+        entropy = torch.empty_like(logprob)
         stats = torch.empty(*lead, 2, dtype=torch.float32, device=dev)
         best = torch.empty(*lead, top, dtype=torch.float32, device=dev) if top else None
-        ids = torch.empty(*lead, top, dtype=torch.int32, device=dev) if top else None
+        ids = torch.empty_like(best, dtype=torch.int32) if top else None
         status = torch.zeros(1, dtype=torch.int32, device=dev) if check_tokens else None
         d = capi.logprobs_desc(z.shape[0], V, z.stride(0), 0, DTYPES[z.dtype], ignore_index, top)
         ws = workspace(capi.logprobs_workspace_size(d), logits)
@@ -58,7 +58,7 @@ def token_logprobs_backward(logits, tokens, stats, entropy, grad_logprob, grad_e
     gl = optional(grad_logprob, "grad_logprob", logits, torch.float32, lead)
     ge = optional(grad_entropy, "grad_entropy", logits, torch.float32, lead)
     with guard(logits):
-        g = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        g = like(logits)
         d = capi.logprobs_desc(z.shape[0], logits.shape[-1], z.stride(0), 0, DTYPES[z.dtype], ignore_index, 0)
         capi.logprobs_bwd(d, z.data_ptr(), t.data_ptr(), stats.data_ptr(), ptr(entropy), ptr(gl), ptr(ge),
                           g.data_ptr(), stream(logits))
