@@ -59,12 +59,23 @@ struct Sums {
         t += o.t;
     }
 };
-__device__ __forceinline__ Sums shfl_sums(const Sums& x, int o) {
-    Sums r;
-    r.m = __shfl_xor(x.m, o, 64);
-    r.s = __shfl_xor(x.s, o, 64);
-    r.t = __shfl_xor(x.t, o, 64);
-    return r;
+// The sums of all lanes, in every lane.
+__device__ __forceinline__ Sums join_wave(Sums x, int lane) {
+    auto with = [&](auto o) {
+        constexpr int O = decltype(o)::value;
+        Sums r;
+        r.m = __uint_as_float(lane_xor<O>(__float_as_uint(x.m), lane));
+        r.s = __uint_as_float(lane_xor<O>(__float_as_uint(x.s), lane));
+        r.t = __uint_as_float(lane_xor<O>(__float_as_uint(x.t), lane));
+        x.join(r);
+    };
+    with(std::integral_constant<int, 32>{});
+    with(std::integral_constant<int, 16>{});
+    with(std::integral_constant<int, 8>{});
+    with(std::integral_constant<int, 4>{});
+    with(std::integral_constant<int, 2>{});
+    with(std::integral_constant<int, 1>{});
+    return x;
 }
 
 // Value and place as a key: larger values first, then lower places.  0: none.
@@ -79,30 +90,31 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t place_of(uint64_t key) { return ~(uint32_t)key; }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t x, int o) {
-    const uint32_t lo = __shfl_xor((uint32_t)x, o, 64), hi = __shfl_xor((uint32_t)(x >> 32), o, 64);
+template <int O> __device__ __forceinline__ uint64_t key_xor(uint64_t x, int lane) {
+    const uint32_t lo = lane_xor<O>((uint32_t)x, lane), hi = lane_xor<O>((uint32_t)(x >> 32), lane);
     return (uint64_t)hi << 32 | lo;
 }
-// Bitonic keys of a wave in falling order.
-__device__ __forceinline__ uint64_t sort_bitonic(uint64_t x, int lane) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint64_t y = shfl_xor64(x, o);
-        x = ((lane & o) == 0) == (x > y) ? x : y;
-    }
+// Lanes O apart in order, the larger first where `falling`.
+template <int O> __device__ __forceinline__ uint64_t exchange(uint64_t x, int lane, bool falling) {
+    const uint64_t y = key_xor<O>(x, lane);
+    return (((lane & O) == 0) == falling) == (x > y) ? x : y;
+}
+// Runs of 2 N lanes that are bitonic, in falling order or (`falling` false in some lanes' run) rising.
+template <int N> __device__ __forceinline__ uint64_t sort_runs(uint64_t x, int lane, bool falling) {
+    x = exchange<N>(x, lane, falling);
+    if constexpr (N > 1) x = sort_runs<N / 2>(x, lane, falling);
     return x;
 }
+// Bitonic keys of a wave in falling order.
+__device__ __forceinline__ uint64_t sort_bitonic(uint64_t x, int lane) { return sort_runs<32>(x, lane, true); }
 // The wave's keys in falling order.
 __device__ __forceinline__ uint64_t sort_wave(uint64_t x, int lane) {
-#pragma unroll
-    for (int n = 2; n <= 64; n *= 2)
-#pragma unroll
-        for (int o = n / 2; o > 0; o >>= 1) {
-            const uint64_t y = shfl_xor64(x, o);
-            const bool falling = n == 64 || (lane & n) == 0;
-            x = (((lane & o) == 0) == falling) == (x > y) ? x : y;
-        }
-    return x;
+    x = sort_runs<1>(x, lane, (lane & 2) == 0);
+    x = sort_runs<2>(x, lane, (lane & 4) == 0);
+    x = sort_runs<4>(x, lane, (lane & 8) == 0);
+    x = sort_runs<8>(x, lane, (lane & 16) == 0);
+    x = sort_runs<16>(x, lane, (lane & 32) == 0);
+    return sort_runs<32>(x, lane, true);
 }
 // The 64 largest of a list in falling order and of other[0 .. n - 1], in falling order as well.
 __device__ __forceinline__ uint64_t merge_list(uint64_t x, const uint64_t* other, int n, int lane) {
@@ -205,8 +217,7 @@ __global__ __launch_bounds__(kLpThreads) void lp_fwd(LogprobsArgs a) {
         if (x == x) best = max(best, key_of(x, (uint32_t)(lo + rest_at(tid))));
     }
 
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) r.join(shfl_sums(r, o));
+    r = join_wave(r, lane);
     if (lane == 0) sm[w] = r.m, ss[w] = r.s, st[w] = r.t;
     if constexpr (TOP) {
         if (tid == 0) n_owners = n_cand = 0;
@@ -260,7 +271,7 @@ __global__ __launch_bounds__(kLpThreads) void lp_fwd(LogprobsArgs a) {
             if (got > kCand - kRound || i0 + NT >= items) {
                 if (w == 0)
                     for (int c = 0; c < got; c += 64) {
-                        const uint64_t y = sort_wave(c + lane < got ? cand[c + lane] : 0, lane), z = shfl_xor64(y, 63);
+                        const uint64_t y = sort_wave(c + lane < got ? cand[c + lane] : 0, lane), z = key_xor<63>(y, lane);
                         list = sort_bitonic(list > z ? list : z, lane);
                     }
                 __syncthreads();
@@ -279,9 +290,11 @@ __global__ __launch_bounds__(kLpThreads) void lp_fwd(LogprobsArgs a) {
     }
 }
 
-// The parts of a row (at most 64: one per lane).
-template <typename T> __global__ __launch_bounds__(kLpThreads) void lp_join(LogprobsArgs a) {
-    __shared__ uint64_t lists[kLpWaves][64];
+// The parts of a row (at most 64: one per lane).  16 waves merge the parts' lists
+// in turn, then each other's.
+constexpr int kJoinWaves = 16;
+template <typename T> __global__ __launch_bounds__(64 * kJoinWaves) void lp_join(LogprobsArgs a) {
+    __shared__ uint64_t lists[kJoinWaves][64];
     const int64_t n = blockIdx.x;
     const int lane = threadIdx.x & 63, w = wave_id();
     if (a.tokens[n] == a.ignore) {
@@ -291,12 +304,14 @@ template <typename T> __global__ __launch_bounds__(kLpThreads) void lp_join(Logp
     uint64_t list = 0;
     if (a.top > 0) {
         const uint64_t* keys = a.part_keys + n * a.parts * a.top;
-        for (int i = w; i < a.parts; i += kLpWaves) list = merge_list(list, keys + i * a.top, a.top, lane);
+        for (int i = w; i < a.parts; i += kJoinWaves)
+            list = i == w ? (lane < a.top ? keys[i * a.top + lane] : 0) : merge_list(list, keys + i * a.top, a.top, lane);
         lists[w][lane] = list;
-        __syncthreads();
-        if (w == 0)
 #pragma unroll
-            for (int i = 1; i < kLpWaves; ++i) list = merge_list(list, lists[i], 64, lane);
+        for (int half = kJoinWaves / 2; half > 0; half /= 2) {
+            __syncthreads();
+            if (w < half) lists[w][lane] = list = merge_list(list, lists[w + half], 64, lane);
+        }
     }
     if (w != 0) return;
     Sums r;
@@ -304,8 +319,7 @@ template <typename T> __global__ __launch_bounds__(kLpThreads) void lp_join(Logp
         const float4 p = a.part[n * a.parts + lane];
         r.m = p.x, r.s = p.y, r.t = p.z;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) r.join(shfl_sums(r, o));
+    r = join_wave(r, lane);
     finish_row<T>(a, n, r, list, lane);
 }
 
@@ -364,7 +378,7 @@ template <typename T> hipError_t fwd(const LogprobsArgs& a, hipStream_t st) {
         else hipLaunchKernelGGL((lp_fwd<T, false, true>), grid, block, 0, st, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((lp_join<T>), dim3((unsigned)a.N), block, 0, st, a);
+        hipLaunchKernelGGL((lp_join<T>), dim3((unsigned)a.N), dim3(64 * kJoinWaves), 0, st, a);
     } else if (a.top) {
         hipLaunchKernelGGL((lp_fwd<T, true, false>), grid, block, 0, st, a);
     } else {

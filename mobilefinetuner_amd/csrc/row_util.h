@@ -4,6 +4,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "attn_common.h"
 
 namespace mft {
@@ -68,6 +70,31 @@ __device__ __forceinline__ float wave_max_f(float x) {
     x = fmaxf(x, dpp<0x140>(x));
     x = row16_max(x);
     return half_max(x);
+}
+
+
+// x of lane (lane ^ O), in registers: quads, halves and rows of 16 by DPP, the
+// rest by lane swaps.  All lanes must be active.
+template <int O> __device__ __forceinline__ uint32_t lane_xor(uint32_t x, int lane) {
+    auto dpp_u = [](uint32_t v, auto ctrl) {
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, true);
+    };
+    if constexpr (O == 1) return dpp_u(x, std::integral_constant<int, 0xB1>{});
+    if constexpr (O == 2) return dpp_u(x, std::integral_constant<int, 0x4E>{});
+    if constexpr (O == 3) return dpp_u(x, std::integral_constant<int, 0x1B>{});
+    if constexpr (O == 7) return dpp_u(x, std::integral_constant<int, 0x141>{});
+    if constexpr (O == 4) return lane_xor<3>(lane_xor<7>(x, lane), lane);
+    if constexpr (O == 8) return dpp_u(x, std::integral_constant<int, 0x128>{});   // row_ror 8
+    if constexpr (O == 15) return dpp_u(x, std::integral_constant<int, 0x140>{});  // row_mirror
+    if constexpr (O == 16) {
+        const auto s = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        return lane & 16 ? s[0] : s[1];
+    }
+    if constexpr (O == 32) {
+        const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return lane & 32 ? s[0] : s[1];
+    }
+    if constexpr (O == 63) return lane_xor<32>(lane_xor<16>(lane_xor<15>(x, lane), lane), lane);
 }
 
 }  // namespace mft
