@@ -14,6 +14,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_kernels.h"
 #include "layer_norm_kernels.h"
@@ -153,21 +154,38 @@ template <typename T> __global__ __launch_bounds__(kLongThreads) void ln_fwd_lon
     }
 }
 
-// Workgroup g: rows in steps of groups * (rows a workgroup holds at once).
-template <typename T, int WPR, int CH, bool PARAMS>
-__global__ __launch_bounds__(kThreads<WPR>) void ln_bwd(LayerNormArgs a) {
-    constexpr int V = kVec<T>, TPR = 64 * WPR, RPB = kThreads<WPR> / TPR;
-    extern __shared__ float lds[];  // PARAMS and RPB > 1: [2][D]
+// Waves of a backward workgroup: eight rows at once, or one row's waves.
+template <int WPR> constexpr int kBwdThreads = WPR == 1 ? 512 : 64 * WPR;
+
+// Workgroup g: rows in steps of groups * (rows a workgroup holds at once).  EVEN:
+// D is a multiple of the vector, so that no element is looked at by itself.
+// Keeping the next row's loads in flight as well takes more registers than it is
+// worth: 16384 x 1024 in bf16 43 us, without and with 16 waves to a CU 31, and 20
+// (4.9 TB/s) since the waves' sums meet in LDS by quads, in pairs of waves.
+template <typename T, int WPR, int CH, bool PARAMS, bool EVEN>
+__global__ __launch_bounds__(kBwdThreads<WPR>) void ln_bwd(LayerNormArgs a) {
+    constexpr int V = kVec<T>, TPR = 64 * WPR, NT = kBwdThreads<WPR>, RPB = NT / TPR;
+    __shared__ __attribute__((aligned(16))) float lds[PARAMS && RPB > 1 ? RPB * CH * V * 64 : 1];
     __shared__ float s[2][2 * WPR];
     const int t = threadIdx.x % TPR;
     const float inv = 1.0f / (float)a.D;
+    // Elements from d0 on, 0 past the row's end (and with it all below).
+    auto load = [&](auto* row, int64_t d0, float* x) {
+        typedef std::remove_const_t<std::remove_pointer_t<decltype(row)>> E;
+        if constexpr (EVEN) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = 0.f;
+            if (d0 < a.D) AnyVec<E, V>::load(row + d0, x);
+        } else {
+            load_part<E, V>(row, d0, a.D, x);
+        }
+    };
     float dw[CH][V], db[CH][V], w[CH][V];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int64_t d0 = (int64_t)(c * TPR + t) * V;
 #pragma unroll
         for (int e = 0; e < V; ++e) dw[c][e] = db[c][e] = 0.f, w[c][e] = 1.f;
-        if (a.w) load_part<float, V>(a.w, d0, a.D, w[c]);
+        if (a.w) load(a.w, (int64_t)(c * TPR + t) * V, w[c]);
     }
     int turn = 0;
     for (int64_t n = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; n < a.N; n += a.groups * RPB) {
@@ -176,9 +194,8 @@ __global__ __launch_bounds__(kThreads<WPR>) void ln_bwd(LayerNormArgs a) {
         float h[CH][V], g[CH][V];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int64_t d0 = (int64_t)(c * TPR + t) * V;
-            load_part<T, V>(xr, d0, a.D, h[c]);
-            load_part<T, V>(gr, d0, a.D, g[c]);  // 0 past the end, and with it all below
+            load(xr, (int64_t)(c * TPR + t) * V, h[c]);
+            load(gr, (int64_t)(c * TPR + t) * V, g[c]);
         }
         const float mean = a.mean_in[n], rstd = a.rstd_in[n];
         float c1 = 0.f, c2 = 0.f;
@@ -207,28 +224,43 @@ __global__ __launch_bounds__(kThreads<WPR>) void ln_bwd(LayerNormArgs a) {
                 if (d0 >= a.D) break;
 #pragma unroll
                 for (int e = 0; e < V; ++e) g[c][e] = rstd * (g[c][e] - c1 - h[c][e] * c2);
-                store_part<T, V>(dr, d0, a.D, g[c]);
+                if constexpr (EVEN) AnyVec<T, V>::store(dr + d0, g[c]);
+                else store_part<T, V>(dr, d0, a.D, g[c]);
             }
         }
     }
     if constexpr (PARAMS) {
         float* out = a.part + (int64_t)blockIdx.x * 2 * a.D;
-        if constexpr (RPB > 1) {  // the waves add in turn
-            for (int i = 0; i < RPB; ++i) {
-                if (threadIdx.x / TPR == i)
+        if constexpr (RPB > 1) {
+            // The waves' sums meet in pairs, half of the waves handing theirs over at a time: quads of
+            // columns, lane by lane, so that no bank is met twice.
+            constexpr int QUADS = 2 * CH * V / 4, SLOT = QUADS * 64 * 4;  // floats of a wave: dw, then db
+            const int wave = threadIdx.x / 64;
+            auto quad = [&](int q) { return q < QUADS / 2 ? &dw[0][0] + 4 * q : &db[0][0] + 4 * (q - QUADS / 2); };
 #pragma unroll
-                    for (int c = 0; c < CH; ++c)
+            for (int half = RPB / 2; half > 0; half /= 2) {
+                if (wave >= half && wave < 2 * half)
 #pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            const int64_t d = (int64_t)(c * TPR + t) * V + e;
-                            if (d < a.D) {
-                                lds[d] = dw[c][e] + (i ? lds[d] : 0.f);
-                                lds[a.D + d] = db[c][e] + (i ? lds[a.D + d] : 0.f);
-                            }
-                        }
+                    for (int q = 0; q < QUADS; ++q)
+                        *reinterpret_cast<f32x4*>(lds + (wave - half) * SLOT + (q * 64 + t) * 4) =
+                            f32x4{quad(q)[0], quad(q)[1], quad(q)[2], quad(q)[3]};
+                __syncthreads();
+                if (wave < half)
+#pragma unroll
+                    for (int q = 0; q < QUADS; ++q) {
+                        const f32x4 o = *reinterpret_cast<const f32x4*>(lds + wave * SLOT + (q * 64 + t) * 4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) quad(q)[e] += o[e];
+                    }
                 __syncthreads();
             }
-            for (int64_t d = threadIdx.x; d < 2 * a.D; d += kThreads<WPR>) out[d] = lds[d];
+            if (wave == 0)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int64_t d0 = (int64_t)(c * TPR + t) * V;
+                    store_part<float, V>(out, d0, a.D, dw[c]);
+                    store_part<float, V>(out + a.D, d0, a.D, db[c]);
+                }
         } else {
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
@@ -291,21 +323,21 @@ template <typename T> __global__ __launch_bounds__(256) void ln_bwd_columns(Laye
     }
 }
 
-// dw and db: the groups' partials in order.  64 columns to a workgroup; its 16
-// waves take the groups in turn.
+// dw and db: the groups' partials in order.  32 columns (a line) to a workgroup;
+// its 32 rows of threads take the groups in turn.
 __global__ __launch_bounds__(1024) void ln_params(LayerNormArgs a) {
-    __shared__ float s[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane, C = 2 * a.D;
+    __shared__ float s[32][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + x, C = 2 * a.D;
     float v = 0.f;
     if (c < C)
 #pragma unroll 8
-        for (int64_t g = w; g < a.groups; g += 16) v += a.part[g * C + c];
-    s[w][lane] = v;
+        for (int64_t g = y; g < a.groups; g += 32) v += a.part[g * C + c];
+    s[y][x] = v;
     __syncthreads();
-    if (w != 0 || c >= C) return;
+    if (y != 0 || c >= C) return;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += s[i][lane];
+    for (int i = 1; i < 32; ++i) v += s[i][x];
     if (c < a.D) {
         if (a.dw) a.dw[c] = v;
     } else if (a.db) {
@@ -331,13 +363,15 @@ Shape fwd_shape(int64_t D, int vec) {
 }
 Shape bwd_shape(int64_t D, int vec) {
     for (const Shape s : {Shape{1, 1}, {1, 2}, {1, 4}, {4, 2}, {4, 4}, {16, 2}})
-        if (D <= (int64_t)64 * s.wpr * s.ch * vec) return s;
+        if (D <= (int64_t)64 * s.wpr * s.ch * vec && s.ch * vec <= 16 * (s.wpr == 4 ? 2 : 1)) return s;
     return {0, 0};
 }
 int64_t bwd_groups(int64_t N, int64_t D, int vec) {
     const Shape s = bwd_shape(D, vec);
-    const int64_t at_once = s.wpr == 1 ? 4 : 1, most = s.wpr == 16 || s.wpr == 0 ? 1 : 2;
-    return std::max<int64_t>(1, std::min<int64_t>((N + at_once - 1) / at_once, most * device_cus()));
+    const int64_t at_once = s.wpr == 1 ? 8 : 1, most = s.wpr == 16 || s.wpr == 0 ? 1 : 2;
+    // few rows, a wave to each: one workgroup to a CU, as each leaves a partial
+    return std::max<int64_t>(1, std::min<int64_t>((N + at_once - 1) / at_once,
+                                                  (s.wpr == 1 && N < 64 * device_cus() ? 1 : most) * device_cus()));
 }
 size_t up(size_t x) { return (x + 255) & ~size_t(255); }
 
@@ -373,23 +407,32 @@ template <typename T> hipError_t bwd(const LayerNormArgs& a, hipStream_t st) {
         hipLaunchKernelGGL((ln_bwd_columns<T>), dim3((unsigned)((a.D + 255) / 256), (unsigned)a.groups), dim3(256), 0,
                            st, q);
     }
+#define MFT_LN_BWD_E(WPR, CH, PARAMS)                                                                           \
+    do {                                                                                                        \
+        if (a.D % kVec<T> == 0)                                                                                 \
+            hipLaunchKernelGGL((ln_bwd<T, WPR, CH, PARAMS, true>), grid, dim3(kBwdThreads<WPR>), 0, st, a);     \
+        else                                                                                                    \
+            hipLaunchKernelGGL((ln_bwd<T, WPR, CH, PARAMS, false>), grid, dim3(kBwdThreads<WPR>), 0, st, a);    \
+    } while (0)
 #define MFT_LN_BWD(WPR, CH)                                                                                     \
     if (s.wpr == WPR && s.ch == CH) {                                                                           \
-        const size_t lds = params && WPR == 1 ? (size_t)a.D * 8 : 0;                                            \
-        const dim3 grid((unsigned)a.groups), block(kThreads<WPR>);                                              \
-        if (params) hipLaunchKernelGGL((ln_bwd<T, WPR, CH, true>), grid, block, (unsigned)lds, st, a);          \
-        else hipLaunchKernelGGL((ln_bwd<T, WPR, CH, false>), grid, block, 0, st, a);                            \
+        if (params) MFT_LN_BWD_E(WPR, CH, true);                                                                \
+        else MFT_LN_BWD_E(WPR, CH, false);                                                                      \
     }
+    const dim3 grid((unsigned)a.groups);
     MFT_LN_BWD(1, 1)
     MFT_LN_BWD(1, 2)
-    MFT_LN_BWD(1, 4)
+    if constexpr (kVec<T> == 4) {
+        MFT_LN_BWD(1, 4)
+    }
     MFT_LN_BWD(4, 2)
     MFT_LN_BWD(4, 4)
     MFT_LN_BWD(16, 2)
+#undef MFT_LN_BWD_E
 #undef MFT_LN_BWD
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !params) return e;
-    hipLaunchKernelGGL(ln_params, dim3((unsigned)((2 * a.D + 63) / 64)), dim3(1024), 0, st, a);
+    hipLaunchKernelGGL(ln_params, dim3((unsigned)((2 * a.D + 31) / 32)), dim3(1024), 0, st, a);
     return hipGetLastError();
 }
 
