@@ -55,13 +55,14 @@ struct Args {
 
 __device__ __forceinline__ constexpr int swz_kc(int r) { return (r >> 1) & 7; }  // 16 rows' reads of a chunk: 16 banks' groups
 
-// One operand of R rows a tile.
-template <int R, bool KC> struct Operand {
-    static constexpr int kSlabBytes = KC ? R * kSlab * 2 : R * kHalf * 2, kRing = KC ? 2 : 3;
-    static constexpr int kBytes = kRing * kSlabBytes;
+// One operand of R rows a tile, for a workgroup of W waves: RING slabs of SK k.
+template <int R, bool KC, int W = 4, int SK = KC ? kSlab : kHalf, int RING = KC ? 2 : 3> struct Operand {
+    static_assert(!KC || SK == kSlab, "whole lines");
+    static_assert(KC || R * 4 % (64 * W) == 0, "every thread's chunks are rows of the slab");
+    static constexpr int kSlabBytes = R * SK * 2, kBytes = RING * kSlabBytes;
     static constexpr int ROW = KC ? kSlab : R, CPR = ROW / 8;  // elements and chunks of an LDS row
-    static constexpr int PER = kSlabBytes / 4096;              // direct loads (1 KiB) of a wave per slab
-    static constexpr int HALF = R / 64;                        // 16-byte chunks of a thread per half
+    static constexpr int PER = kSlabBytes / 1024 / W;          // direct loads (1 KiB) of a wave per slab
+    static constexpr int HALF = (R * 4 + 64 * W - 1) / (64 * W);  // 16-byte chunks of a thread per half, at most
     // The slab that holds half h (an offset in the operand's LDS).
     __device__ __forceinline__ static int slab(int h) {
         return KC ? (h >> 1 & 1) * kSlabBytes : (int)((unsigned)h % 3u) * kSlabBytes;
@@ -72,14 +73,14 @@ template <int R, bool KC> struct Operand {
     struct Dma {
         uint32_t off[PER];
         __device__ __forceinline__ void init(int w, int lane, int64_t r0, int64_t rows, int64_t ld) {
-            static_assert(PER * 4096 == kSlabBytes && 64 % CPR == 0, "whole loads of whole rows");
+            static_assert(PER * W * 1024 == kSlabBytes && 64 % CPR == 0, "whole loads of whole rows");
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
                 const int r = (w * PER + j) * (64 / CPR) + lane / CPR, c = lane % CPR ^ swz_of(r);
                 if (KC)  // rows past the end are read again from the last one, and not stored
                     off[j] = (uint32_t)((min(r0 + r, rows - 1) - r0) * ld * 2) + 16u * c;
                 else
-                    off[j] = (uint32_t)(r * ld * 2) + (uint32_t)(min(r0 + 8 * c, rows - 8) - r0) * 2u;
+                    off[j] = (uint32_t)(r * ld * 2) + (uint32_t)(min(r0 + 8 * c, (rows - 1) / 8 * 8) - r0) * 2u;  // rows are of whole chunks
             }
         }
         // Load j of the slab whose first element is `from`, into the slab at LDS address `to`.
@@ -90,8 +91,8 @@ template <int R, bool KC> struct Operand {
 
     // A half through registers, from anywhere and with zeros past the ends.
     typedef bf16 any8 __attribute__((ext_vector_type(8), aligned(2)));
-    __device__ __forceinline__ static int half_row(int j, int tid) { return KC ? (j * kThreads + tid) / 4 : (j * kThreads + tid) / CPR; }
-    __device__ __forceinline__ static int half_chunk(int j, int tid) { return KC ? tid % 4 : (j * kThreads + tid) % CPR; }
+    __device__ __forceinline__ static int half_row(int j, int tid) { return (j * 64 * W + tid) / (KC ? 4 : CPR); }
+    __device__ __forceinline__ static int half_chunk(int j, int tid) { return (j * 64 * W + tid) % (KC ? 4 : CPR); }
     __device__ __forceinline__ static bf16x8 fetch(const bf16* p, int64_t ld, int64_t r0, int64_t rows, int64_t k0,
                                                    int64_t K, int j, int tid) {
         const int r = half_row(j, tid), c = half_chunk(j, tid);
@@ -109,9 +110,11 @@ template <int R, bool KC> struct Operand {
         }
         return v;
     }
-    __device__ __forceinline__ static void store(char* lds, int h, int j, int tid, bf16x8 v) {  // h even
-        const int r = half_row(j, tid), c = half_chunk(j, tid);
-        *reinterpret_cast<bf16x8*>(lds + slab(h) + r * ROW * 2 + (c ^ swz_of(r)) * 16) = v;
+    // The first half of the slab at `to`, or with SK = 64 the second one.
+    __device__ __forceinline__ static void store(char* to, int second, int j, int tid, bf16x8 v) {
+        if (R * 4 % (64 * W) != 0 && j * 64 * W + tid >= R * 4) return;
+        const int r = half_row(j, tid) + (KC ? 0 : kHalf * second), c = half_chunk(j, tid) + (KC ? 4 * second : 0);
+        *reinterpret_cast<bf16x8*>(to + r * ROW * 2 + (c ^ swz_of(r)) * 16) = v;
     }
 };
 
@@ -147,6 +150,50 @@ template <int R, bool KC, int T> struct Fragments {
     static constexpr int kReads = KC ? T : 2 * T;
 };
 
+// This workgroup's slice and tile.
+template <int BN, int BM> __device__ __forceinline__ void place(const Args& a, int* slice, int64_t* m0, int64_t* n0) {
+    int i = xcd_block((int)blockIdx.x, (int)gridDim.x);
+    *slice = __builtin_amdgcn_readfirstlane((int)a.per_slice_tiles.div(i));
+    i -= *slice * a.tiles_m * a.tiles_n;
+    // Eight rows of tiles at a time, column by column.
+    constexpr int kBand = 8;
+    const int band = i / (kBand * a.tiles_n), in = i - band * kBand * a.tiles_n;
+    const int high = min(kBand, a.tiles_m - band * kBand), col = in / high;
+    // scalars, whatever unit divides: the direct loads take their bases from them
+    *n0 = (int64_t)__builtin_amdgcn_readfirstlane(col) * BN;
+    *m0 = (int64_t)__builtin_amdgcn_readfirstlane(band * kBand + in - col * high) * BM;
+}
+
+// 32 rows of C from mw on, 32 TN columns from nw on, through this wave's LDS (32
+// rows of 32 TN + 4 fp32: a bank group apart).
+template <int TN, int ACT>
+__device__ __forceinline__ void write_rows(const Args& a, int slice, int64_t mw, int64_t nw, const f32x16 (&acc)[TN],
+                                           float* st, int lane) {
+    constexpr int V = 8, LPR = 32 * TN / V, kPitch = 32 * TN + 4;  // lanes to a row
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f32x4*>(st + (lane & 31) * kPitch + 32 * j + 8 * q + 4 * (lane >> 5)) =
+                f32x4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
+    asm volatile("" ::: "memory");  // a wave's LDS accesses stay in order
+#pragma unroll
+    for (int r = 0; r < LPR / 2; ++r) {
+        const int at = r * 64 + lane, row = at / LPR, c = at % LPR * V;
+        const int64_t m = mw + row, n = nw + c;
+        if (m >= a.g.M || n >= a.g.N) continue;
+        float v[V];
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+            const f32x4 u = *reinterpret_cast<const f32x4*>(st + row * kPitch + c + e);
+            v[e] = u[0], v[e + 1] = u[1], v[e + 2] = u[2], v[e + 3] = u[3];
+        }
+        if (a.whole) linear_epilogue<bf16, ACT, V>(a.g, m, n, v);
+        else store_part<float, V>(a.g.partial + ((int64_t)slice * a.g.M + m) * a.g.N, n, a.g.N, v);
+    }
+    asm volatile("" ::: "memory");
+}
+
 template <int BN, int BM, bool PKC, bool QKC, bool DMA, int ACT>
 __global__ __launch_bounds__(kThreads, BN * BM > 32768 ? 1 : 2) void bf_gemm_kernel(Args a) {
     constexpr int TN = BN / 64, TM = BM / 64;  // 32 x 32 tiles of a wave
@@ -159,21 +206,14 @@ __global__ __launch_bounds__(kThreads, BN * BM > 32768 ? 1 : 2) void bf_gemm_ker
     const int lane = threadIdx.x & 63, w = wave_id(), hh = lane >> 5;
     const int wn = w & 1, wm = w >> 1;
 
-    int i = xcd_block((int)blockIdx.x, (int)gridDim.x);
-    const int slice = __builtin_amdgcn_readfirstlane((int)a.per_slice_tiles.div(i));
-    i -= slice * a.tiles_m * a.tiles_n;
-    // Eight rows of tiles at a time, column by column.
-    constexpr int kBand = 8;
-    const int band = i / (kBand * a.tiles_n), in = i - band * kBand * a.tiles_n;
-    const int high = min(kBand, a.tiles_m - band * kBand), col = in / high;
-    // scalars, whatever unit divides: the direct loads take their bases from them
-    const int tn = __builtin_amdgcn_readfirstlane(col), tm = __builtin_amdgcn_readfirstlane(band * kBand + in - col * high);
-    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    int slice;
+    int64_t m0, n0;
+    place<BN, BM>(a, &slice, &m0, &n0);
     const bool last = slice == a.slices - 1;
     // Halves of this slice, and where the last one's k end (the rest of K goes through registers).
     const int h0 = slice * a.per_slice, h1 = last ? a.halves : h0 + a.per_slice;
 
-    const int64_t ldp = PKC ? a.g.K : a.g.M, ldq = QKC ? a.g.K : a.g.N;
+    const int64_t ldp = a.g.ldp, ldq = a.g.ldq;
     const bf16 *P = (const bf16*)a.g.P, *Q = (const bf16*)a.g.Q;
     Fragments<BM, PKC, TM> fp;
     Fragments<BN, QKC, TN> fq;
@@ -327,9 +367,9 @@ __global__ __launch_bounds__(kThreads, BN * BM > 32768 ? 1 : 2) void bf_gemm_ker
             // have read the one before the last.
             const int i = 2 * (h - from);
 #pragma unroll
-            for (int j = 0; j < OpQ::HALF; ++j) OpQ::store(smem, i, j, threadIdx.x, rq[j]);
+            for (int j = 0; j < OpQ::HALF; ++j) OpQ::store(smem + OpQ::slab(i), 0, j, threadIdx.x, rq[j]);
 #pragma unroll
-            for (int j = 0; j < OpP::HALF; ++j) OpP::store(lds_p, i, j, threadIdx.x, rp[j]);
+            for (int j = 0; j < OpP::HALF; ++j) OpP::store(lds_p + OpP::slab(i), 0, j, threadIdx.x, rp[j]);
             lds_barrier();
             if (h + 1 < to) fetch(h + 1);
 #pragma unroll
@@ -337,38 +377,196 @@ __global__ __launch_bounds__(kThreads, BN * BM > 32768 ? 1 : 2) void bf_gemm_ker
         }
     }
 
-    // The accumulators, 32 rows of m at a time, through this wave's part of LDS.
     lds_barrier();
     float* st = reinterpret_cast<float*>(smem) + w * 32 * kPitch;
-    constexpr int V = 8, LPR = WN / V;  // lanes to a row
-    const int64_t nw = n0 + wn * WN;
 #pragma unroll
     for (int k = 0; k < TM; ++k) {
         const int64_t mw = m0 + wm * (BM / 2) + 32 * k;
         if (mw >= a.g.M) break;
+        f32x16 rows[TN];
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<f32x4*>(st + (lane & 31) * kPitch + 32 * j + 8 * q + 4 * hh) =
-                    f32x4{acc[j][k][4 * q], acc[j][k][4 * q + 1], acc[j][k][4 * q + 2], acc[j][k][4 * q + 3]};
-        asm volatile("" ::: "memory");  // a wave's LDS accesses stay in order
-#pragma unroll
-        for (int r = 0; r < LPR / 2; ++r) {
-            const int at = r * 64 + lane, row = at / LPR, c = at % LPR * V;
-            const int64_t m = mw + row, n = nw + c;
-            if (m >= a.g.M || n >= a.g.N) continue;
-            float v[V];
-#pragma unroll
-            for (int e = 0; e < V; e += 4) {
-                const f32x4 u = *reinterpret_cast<const f32x4*>(st + row * kPitch + c + e);
-                v[e] = u[0], v[e + 1] = u[1], v[e + 2] = u[2], v[e + 3] = u[3];
-            }
-            if (a.whole) linear_epilogue<bf16, ACT, V>(a.g, m, n, v);
-            else store_part<float, V>(a.g.partial + ((int64_t)slice * a.g.M + m) * a.g.N, n, a.g.N, v);
-        }
-        asm volatile("" ::: "memory");
+        for (int j = 0; j < TN; ++j) rows[j] = acc[j][k];
+        write_rows<TN, ACT>(a, slice, mw, n0 + wn * WN, rows, st, lane);
     }
+}
+
+// A tile for a CU of its own: two groups of 2 x 2 waves take the halves of each
+// pair of halves, three or four pairs are in LDS, and the groups' sums meet there
+// at the end.
+constexpr int kDeepThreads = 512;
+template <int BN, int BM, bool PKC, bool QKC, bool DMA, int ACT>
+__global__ __launch_bounds__(kDeepThreads, 2) void bf_gemm_deep(Args a) {
+    constexpr int TN = BN / 64, TM = BM / 64, kTiles = TN * TM, kFrags = TN + TM;
+    static_assert(TM == 2, "each group writes one of a wave's two rows of tiles");
+    constexpr int kRing = (160 << 10) / ((BN + BM) * kSlab * 2) < 4 ? 3 : 4;
+    typedef Operand<BM, PKC, 8, kSlab, kRing> OpP;
+    typedef Operand<BN, QKC, 8, kSlab, kRing> OpQ;
+    constexpr int kPair = OpQ::kSlabBytes + OpP::kSlabBytes, PER = OpQ::PER + OpP::PER;
+    constexpr int kPitch = 32 * TN + 4;
+    static_assert(8 * 32 * kPitch * 4 <= kRing * kPair && 8 * TN * 16 * 64 * 4 <= kRing * kPair, "fits the slabs");
+    __shared__ __attribute__((aligned(1024))) char smem[kRing * kPair];  // [pair][Q, P]
+    const int lane = threadIdx.x & 63, w = wave_id();
+    const int wn = w & 1, wm = w >> 1 & 1, group = w >> 2;
+    int slice;
+    int64_t m0, n0;
+    place<BN, BM>(a, &slice, &m0, &n0);
+    const int p0 = slice * a.per_slice / 2, p1 = min(p0 + a.per_slice / 2, a.halves / 2);  // pairs
+    const int64_t ldp = a.g.ldp, ldq = a.g.ldq;
+    const bf16 *P = (const bf16*)a.g.P, *Q = (const bf16*)a.g.Q;
+    Fragments<BM, PKC, TM> fp;
+    Fragments<BN, QKC, TN> fq;
+    fp.init(wm * BM / 2, lane);
+    fq.init(wn * BN / 2, lane);
+    // This group's half of a slab.
+    const int half_p = group * (PKC ? 0 : OpP::kSlabBytes / 2), half_q = group * (QKC ? 0 : OpQ::kSlabBytes / 2);
+    if (PKC && group)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) fp.at[i] = fp.at[2 + i];
+    if (QKC && group)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) fq.at[i] = fq.at[2 + i];
+    f32x16 acc[TN][TM];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int k = 0; k < TM; ++k) {
+            acc[j][k] = zero16();
+            asm volatile("" : "+v"(acc[j][k]));  // not a literal zero (see mfma_v_first)
+        }
+    struct Ops {
+        bf16x8 q[TN], p[TM];
+    };
+    auto read_one = [&](Ops& o, int slot, int ks, int f) {
+        const char* at = smem + slot * kPair;
+        if (f < TM) o.p[f] = fp.read(at + OpQ::kSlabBytes + half_p, false, ks, f);
+        else o.q[f - TM] = fq.read(at + half_q, false, ks, f - TM);
+    };
+    auto read = [&](int slot, int ks) {
+        Ops o;
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f) read_one(o, slot, ks, f);
+        return o;
+    };
+    auto multiply_one = [&](const Ops& o, int t) { acc[t / TM][t % TM] = mfma_bf16(o.q[t / TM], o.p[t % TM], acc[t / TM][t % TM]); };
+    if (DMA && p0 < p1) {
+        typename OpP::Dma dp;
+        typename OpQ::Dma dq;
+        dp.init(w, lane, m0, a.g.M, ldp);
+        dq.init(w, lane, n0, a.g.N, ldq);
+        const char* tp = reinterpret_cast<const char*>(P + (PKC ? m0 * ldp : m0));
+        const char* tq = reinterpret_cast<const char*>(Q + (QKC ? n0 * ldq : n0));
+        const int64_t step_p = (int64_t)kSlab * 2 * (PKC ? 1 : ldp), step_q = (int64_t)kSlab * 2 * (QKC ? 1 : ldq);
+        const uint32_t base = lds_addr(smem);
+        auto issue_one = [&](int p, int slot, int j) {
+            const uint32_t to = base + (uint32_t)(slot * kPair);
+            if (j < OpQ::PER) dq.issue(tq + p * step_q, to, w, j);
+            else dp.issue(tp + p * step_p, to + OpQ::kSlabBytes, w, j - OpQ::PER);
+        };
+#pragma unroll
+        for (int i = 0; i < kRing; ++i)
+            if (p0 + i < p1)
+#pragma unroll
+                for (int j = 0; j < PER; ++j) issue_one(p0 + i, i, j);
+        if (p0 + kRing <= p1) wait_vmcnt<(kRing - 1) * PER>();
+        else wait_vmcnt<0>();
+        lds_barrier();
+        Ops cur = read(0, 0);
+        // MORE: pair p + kRing exists.
+        auto pair = [&](int p, int slot, auto more_t) {
+            constexpr bool MORE = decltype(more_t)::value;
+            const int after = slot + 1 == kRing ? 0 : slot + 1;
+            Ops nxt;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+                for (int f = t * kFrags / kTiles; f < (t + 1) * kFrags / kTiles; ++f) read_one(nxt, slot, 1, f);
+                multiply_one(cur, t);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // Pair p + 1 has landed, and everybody has read pair p.
+            if constexpr (MORE) wait_vmcnt<(kRing - 2) * PER>();
+            else wait_vmcnt<0>();
+            lds_barrier();
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                if (MORE || p + 1 < p1) {
+#pragma unroll
+                    for (int f = t * kFrags / kTiles; f < (t + 1) * kFrags / kTiles; ++f) read_one(cur, after, 0, f);
+                }
+                multiply_one(nxt, t);
+                if constexpr (MORE) {
+#pragma unroll
+                    for (int j = t * PER / kTiles; j < (t + 1) * PER / kTiles; ++j) issue_one(p + kRing, slot, j);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        int p = p0, slot = 0;
+        for (; p + kRing < p1; ++p) {
+            pair(p, slot, std::true_type{});
+            slot = slot + 1 == kRing ? 0 : slot + 1;
+        }
+        for (; p < p1; ++p) {
+            pair(p, slot, std::false_type{});
+            slot = slot + 1 == kRing ? 0 : slot + 1;
+        }
+    }
+    // What is left of K in pairs, or all of it, half by half through registers, the groups in turn.
+    const bool last = slice == a.slices - 1;
+    const int from = DMA ? a.halves : 2 * p0, to = !last ? (DMA ? from : 2 * p1) : (int)((a.g.K + kHalf - 1) / kHalf);
+    bf16x8 rp[OpP::HALF], rq[OpQ::HALF];
+    auto fetch = [&](int h) {
+        const int64_t k0 = (int64_t)h * kHalf;
+#pragma unroll
+        for (int j = 0; j < OpQ::HALF; ++j) rq[j] = OpQ::fetch(Q, ldq, n0, a.g.N, k0, a.g.K, j, threadIdx.x);
+#pragma unroll
+        for (int j = 0; j < OpP::HALF; ++j) rp[j] = OpP::fetch(P, ldp, m0, a.g.M, k0, a.g.K, j, threadIdx.x);
+    };
+    if (from < to) fetch(from);
+    for (int h = from; h < to; ++h) {
+        lds_barrier();  // everybody has read what was there
+#pragma unroll
+        for (int j = 0; j < OpQ::HALF; ++j) OpQ::store(smem, h & 1, j, threadIdx.x, rq[j]);
+#pragma unroll
+        for (int j = 0; j < OpP::HALF; ++j) OpP::store(smem + OpQ::kSlabBytes, h & 1, j, threadIdx.x, rp[j]);
+        lds_barrier();
+        if (h + 1 < to) fetch(h + 1);
+        if ((h & 1) == group) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const Ops o = read(0, ks);
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) multiply_one(o, t);
+            }
+        }
+    }
+    // Each group hands the other one half of its rows of m.
+    lds_barrier();
+    float* give = reinterpret_cast<float*>(smem) + (w ^ 4) * TN * 16 * 64;
+    const float* got = reinterpret_cast<float*>(smem) + w * TN * 16 * 64;
+    f32x16 rows[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        rows[j] = group ? acc[j][1] : acc[j][0];
+        const f32x16 other = group ? acc[j][0] : acc[j][1];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f32x4*>(give + ((j * 4 + q) * 64 + lane) * 4) =
+                f32x4{other[4 * q], other[4 * q + 1], other[4 * q + 2], other[4 * q + 3]};
+    }
+    lds_barrier();
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 o = *reinterpret_cast<const f32x4*>(got + ((j * 4 + q) * 64 + lane) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rows[j][4 * q + e] += o[e];
+        }
+    lds_barrier();
+    const int64_t mw = m0 + wm * (BM / 2) + 32 * group;
+    if (mw < a.g.M)
+        write_rows<TN, ACT>(a, slice, mw, n0 + wn * (BN / 2), rows, reinterpret_cast<float*>(smem) + w * 32 * kPitch, lane);
 }
 
 // The slices' partial products in their order, then the epilogue.
@@ -397,31 +595,40 @@ struct Plan {
 
 // The tiles, and what each sustains over the whole GPU (TFLOP/s) with one
 // workgroup to a CU and with more, and the k that its prologue and epilogue are
-// worth (with an activation: `act` more).  Fitted to 42 products of 1 to 8192
-// rows and 640 to 6912 columns, each timed in every tile and cut into 1 to 16
-// slices: the choice by these is within 6 percent of the best, but for five, the
-// worst at 1.16 times it.  256 x 256 reads least of LDS and L2 per product, holds
-// its accumulators in all of a SIMD's registers and has nobody to overlap its
-// epilogue with (4096^3, W [out, in]: 112 us, 128 x 128 125; 8192 x 1024 -> 4096
-// with GELU 95, 256 x 128 86).  With k contiguous in both operands the slabs of
-// 256 x 128 do not leave a CU room for two.
+// worth (with an activation: `act` more).  Fitted to 51 products of 16 to 8192
+// rows and 640 to 6912 columns, each timed on operands out of cache in every
+// tile and cut into 1 to 8 slices: the choice by these is the fastest or within 6
+// percent of it but for three, the worst at 1.13 times it.
+//   256 x 128, two workgroups to a CU: heavy epilogues over short K.  8192 x 1024
+//     -> 4096 with GELU 94 us, 256 x 256 104, 128 x 128 112.
+//   256 x 256, one wave to a SIMD with its accumulators in all of its registers:
+//     least LDS and L2 traffic per product.  8192^3 815 us (1350 TFLOP/s), 128 x
+//     128 980.
+//   deep: 8192 x 1024 -> 4096's dW (256 tiles of 128 x 128 over K 8192) 79 us, 104
+//     with one workgroup of 4 waves to a CU; its dx in 256 x 128 63 us for 71 in
+//     128 x 128; 4096 x 6912 -> 1152 in 192 x 128 79 us for 96.
+// With k contiguous in both operands the slabs of 256 x 128 do not leave a CU
+// room for two; a slab of 192 rows has no whole direct loads without.
 struct Shape {
-    int bn, bm;
+    int bn, bm, deep;
     double one, more;
     int k, act;
 };
-constexpr Shape kShapes[] = {{256, 128, 1000, 1350, 330, 190},
-                             {128, 128, 900, 1080, 345, 190},
-                             {64, 64, 400, 760, 200, 100},
-                             {256, 256, 1400, 1400, 640, 200}};
-bool has_shape(const LinearProduct& g, int s) { return s != 0 || (g.p_kc && !g.q_kc); }
+constexpr Shape kShapes[] = {{256, 128, 0, 1000, 1350, 330, 190}, {128, 128, 0, 900, 1080, 345, 190},
+                             {64, 64, 0, 400, 720, 200, 100},     {256, 256, 0, 1400, 1540, 704, 200},
+                             {128, 128, 1, 1200, 1200, 380, 190}, {192, 128, 1, 1200, 1260, 345, 190},
+                             {256, 128, 1, 1520, 1200, 380, 190}};
+constexpr int kShapeCount = sizeof(kShapes) / sizeof(kShapes[0]);
+bool has_shape(const LinearProduct& g, int s) {
+    return s == 0 ? g.p_kc && !g.q_kc : s == 5 ? g.q_kc != 0 : true;
+}
 
 Plan plan(const LinearProduct& g) {
     Plan p{};
     const int cus = device_cus(), pairs = (int)(g.K / kSlab);
     double best = 1e300;
     int per = 1;
-    for (int s = 0; s < 4; ++s) {
+    for (int s = 0; s < kShapeCount; ++s) {
         if (!has_shape(g, s)) continue;
         const Shape& t = kShapes[s];
         const int64_t tiles = ((g.N + t.bn - 1) / t.bn) * ((g.M + t.bm - 1) / t.bm);
@@ -429,10 +636,10 @@ Plan plan(const LinearProduct& g) {
             if (slices > 1 && (slices > pairs || tiles * slices > 4 * cus)) break;
             const int per_slice = std::max(1, (pairs + slices - 1) / slices), n = std::max(1, (pairs + per_slice - 1) / per_slice);
             const double mean = (double)tiles * n / cus, most = std::ceil(mean);
-            const double rate = (most <= 1 ? t.one : t.more) * (g.p_kc && g.q_kc ? 1.1 : 1.0) * cus / 256;
-            double us = (most <= 1 ? 1 : (most + mean) / 2) * cus * t.bn * t.bm * 2 *
+            const double rate = (most <= 1 ? t.one : t.more) * (g.p_kc && g.q_kc ? 1.08 : 1.0) * cus / 256;
+            double us = (most <= 1 ? 1 : t.deep ? most : (most + mean) / 2) * cus * t.bn * t.bm * 2 *
                         ((double)g.K / n + t.k + (g.act != ACT_NONE && n == 1 ? t.act : 0)) / rate / 1e6;
-            if (n > 1) us += 5 + (double)n * g.M * g.N * 8 / 4.5e6;  // partials written and read, a launch
+            if (n > 1) us += 1 + (double)n * g.M * g.N * 8 / 5.4e6;  // partials written and read, a launch
             if (us < best * 0.999) best = us, p.shape = s, per = per_slice;
         }
     }
@@ -453,6 +660,11 @@ template <int BN, int BM, bool PKC, bool QKC, int ACT> void launch_t(const Args&
     if (dma) hipLaunchKernelGGL((bf_gemm_kernel<BN, BM, PKC, QKC, true, ACT>), grid, dim3(kThreads), 0, st, a);
     else hipLaunchKernelGGL((bf_gemm_kernel<BN, BM, PKC, QKC, false, ACT>), grid, dim3(kThreads), 0, st, a);
 }
+template <int BN, bool PKC, bool QKC, int ACT> void launch_deep(const Args& a, bool dma, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)a.tiles_m * a.tiles_n * a.slices));
+    if (dma) hipLaunchKernelGGL((bf_gemm_deep<BN, 128, PKC, QKC, true, ACT>), grid, dim3(kDeepThreads), 0, st, a);
+    else hipLaunchKernelGGL((bf_gemm_deep<BN, 128, PKC, QKC, false, ACT>), grid, dim3(kDeepThreads), 0, st, a);
+}
 template <bool PKC, bool QKC, int ACT> void launch_s(const Plan& p, bool dma, hipStream_t st) {
     if constexpr (PKC && !QKC) {
         if (p.shape == 0) launch_t<256, 128, PKC, QKC, ACT>(p.a, dma, st);
@@ -460,23 +672,87 @@ template <bool PKC, bool QKC, int ACT> void launch_s(const Plan& p, bool dma, hi
     if (p.shape == 1) launch_t<128, 128, PKC, QKC, ACT>(p.a, dma, st);
     if (p.shape == 2) launch_t<64, 64, PKC, QKC, ACT>(p.a, dma, st);
     if (p.shape == 3) launch_t<256, 256, PKC, QKC, ACT>(p.a, dma, st);
+    if (p.shape == 4) launch_deep<128, PKC, QKC, ACT>(p.a, dma, st);
+    if constexpr (QKC) {
+        if (p.shape == 5) launch_deep<192, PKC, QKC, ACT>(p.a, dma, st);
+    }
+    if (p.shape == 6) launch_deep<256, PKC, QKC, ACT>(p.a, dma, st);
 }
 template <int ACT> void launch_act_fwd(const Plan& p, bool dma, hipStream_t st) {
     if (p.a.g.q_kc) launch_s<true, true, ACT>(p, dma, st);
     else launch_s<true, false, ACT>(p, dma, st);
 }
 
-}  // namespace
-
-size_t bf_gemm_workspace(const LinearProduct& g) {
-    const Plan p = plan(g);
-    return p.a.whole ? 0 : (size_t)p.a.slices * g.M * g.N * 4;
+// Operands whose rows are off 16 bytes are first copied to rows of whole ones,
+// where the product (of M N K pairs of numbers) is worth up to two more launches:
+// 5000 x 600 -> 1500 with W [in, out] 38 -> 25 us, its dW 56 -> 29; 300 x 600 ->
+// 1501 17 -> 11.  With k contiguous in the operands that are off, the registers'
+// way is less slow: 300 x 1501 by [600, 1501] 11.5 us, copied 17.
+constexpr double kPackWorth = 1e8, kPackWorthKc = 1.5e9;
+size_t up(size_t x) { return (x + 255) & ~size_t(255); }
+int64_t whole_ld(int64_t cols) { return (cols + 7) / 8 * 8; }
+struct Packs {
+    bool p, q;
+    int64_t rows_p, cols_p, rows_q, cols_q;
+    size_t at_p, at_q, total;
+};
+Packs packs(const LinearProduct& g, const Plan& plan) {
+    Packs k{};
+    k.rows_p = g.p_kc ? g.M : g.K, k.cols_p = g.p_kc ? g.K : g.M;
+    k.rows_q = g.q_kc ? g.N : g.K, k.cols_q = g.q_kc ? g.K : g.N;
+    const bool off_p = k.cols_p % 8 != 0 && g.ldp == 0, off_q = k.cols_q % 8 != 0 && g.ldq == 0;
+    const bool worth = (double)g.M * g.N * g.K >= ((off_p && !g.p_kc) || (off_q && !g.q_kc) ? kPackWorth : kPackWorthKc);
+    k.p = worth && off_p;
+    k.q = worth && off_q;
+    size_t o = plan.a.whole ? 0 : up((size_t)plan.a.slices * g.M * g.N * 4);
+    k.at_p = o, o += k.p ? up((size_t)k.rows_p * whole_ld(k.cols_p) * 2) : 0;
+    k.at_q = o, o += k.q ? up((size_t)k.rows_q * whole_ld(k.cols_q) * 2) : 0;
+    k.total = o;
+    return k;
 }
 
-hipError_t launch_bf_gemm(const LinearProduct& g, hipStream_t st) {
+// rows x cols of bf16 into rows of ld (a multiple of 8), zeros behind them.
+__global__ __launch_bounds__(256) void pack_rows(const bf16* from, bf16* to, int64_t rows, int64_t cols, int64_t ld) {
+    const int64_t chunks = ld / 8, step = (int64_t)gridDim.x * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * chunks; i += step) {
+        const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+        float v[8];
+        load_part<bf16, 8>(from + r * cols, c, cols, v);
+        AnyVec<bf16, 8>::store(to + r * ld + c, v);
+    }
+}
+hipError_t pack(const void* from, void* to, int64_t rows, int64_t cols, hipStream_t st) {
+    const int64_t ld = whole_ld(cols), n = rows * (ld / 8);
+    const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 16 * device_cus()));
+    hipLaunchKernelGGL(pack_rows, grid, dim3(256), 0, st, (const bf16*)from, (bf16*)to, rows, cols, ld);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t bf_gemm_workspace(const LinearProduct& g) { return packs(g, plan(g)).total; }
+
+hipError_t launch_bf_gemm(const LinearProduct& given, hipStream_t st) {
+    LinearProduct g = given;
     if (g.M <= 0 || g.N <= 0 || g.K <= 0) return hipSuccess;
-    const Plan p = plan(g);
-    const int64_t ldp = g.p_kc ? g.K : g.M, ldq = g.q_kc ? g.K : g.N;
+    Plan p = plan(g);
+    const Packs k = packs(g, p);
+    if (g.ldp == 0) g.ldp = k.cols_p;
+    if (g.ldq == 0) g.ldq = k.cols_q;
+    char* ws = reinterpret_cast<char*>(g.partial);
+    if (k.p) {
+        const hipError_t e = pack(g.P, ws + k.at_p, k.rows_p, k.cols_p, st);
+        if (e != hipSuccess) return e;
+        g.P = ws + k.at_p, g.ldp = whole_ld(k.cols_p);
+    }
+    if (k.q) {
+        const hipError_t e = pack(g.Q, ws + k.at_q, k.rows_q, k.cols_q, st);
+        if (e != hipSuccess) return e;
+        g.Q = ws + k.at_q, g.ldq = whole_ld(k.cols_q);
+    }
+    p.a.g = g;
+    const int64_t ldp = g.ldp, ldq = g.ldq;
+    // direct loads take 16 bytes whole, also at the end of a row
     const bool dma = ldp % 8 == 0 && ldq % 8 == 0 && on16(g.P) && on16(g.Q) && ldp <= (1 << 22) && ldq <= (1 << 22);
     // an epilogue after the slices' sum is the reduce kernel's
     const int act = p.a.whole ? g.act : ACT_NONE;

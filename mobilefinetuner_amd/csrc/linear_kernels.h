@@ -11,13 +11,15 @@ namespace mft {
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU_TANH = 2, ACT_SILU = 3 };
 
 // C[M, N] = act(sum_k P(m, k) Q(n, k) + bias[n]) + residual.  P is stored [M, K]
-// (p_kc) or [K, M], Q [N, K] (q_kc) or [K, N], all contiguous; all bf16, or all
-// fp32, but bias (fp32).
+// (p_kc) or [K, M], Q [N, K] (q_kc) or [K, N], contiguous or, in bf16, with rows
+// of ldp and ldq elements; all else contiguous.  All bf16, or all fp32, but bias
+// (fp32).
 struct LinearProduct {
     int64_t M, N, K;
     const void* P;
     const void* Q;
     int p_kc, q_kc;
+    int64_t ldp, ldq;      // 0: contiguous
     void* C;
     // epilogue
     const float* bias;     // [N] or null
