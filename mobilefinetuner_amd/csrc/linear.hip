@@ -75,9 +75,31 @@ __global__ __launch_bounds__(1024) void db_kernel(const float* part, float* db, 
     db[c] = v;
 }
 
+// db[c] = the sums of dy's columns, in one launch: 32 columns to a workgroup, whose
+// 32 rows of threads take dy's rows in turn.  1021 x 2304 in fp32 5 us for 9 as
+// strips and their sums.
+template <typename T>
+__global__ __launch_bounds__(1024) void column_sums(const T* dy, float* db, int64_t N, int64_t out) {
+    __shared__ float s[32][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + x;
+    float v = 0.f;
+    if (c < out)
+#pragma unroll 8
+        for (int64_t n = y; n < N; n += 32) v += (float)dy[n * out + c];
+    s[y][x] = v;
+    __syncthreads();
+    if (y != 0 || c >= out) return;
+#pragma unroll
+    for (int i = 1; i < 32; ++i) v += s[i][x];
+    db[c] = v;
+}
+
 __global__ __launch_bounds__(256) void fill_zero_kernel(uint16_t* p, size_t n) {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = 0;
 }
+
+constexpr int64_t kFewRows = 2048;  // that 32 rows of threads add in a few rounds of loads
 
 // Row strips: about four workgroups a CU, each of at least 32 rows.
 int64_t dz_strips(int64_t N, int64_t out) {
@@ -122,6 +144,12 @@ size_t dz_workspace(int64_t N, int64_t out) { return (size_t)dz_strips(N, out) *
 hipError_t launch_dz(const void* dy, const void* z, void* dz, float* db, int64_t N, int64_t out, int act, bool is_bf16,
                      float* workspace, hipStream_t st) {
     if (act == ACT_NONE && !db) return hipSuccess;
+    if (act == ACT_NONE && N <= kFewRows) {
+        const dim3 grid((unsigned)((out + 31) / 32));
+        if (is_bf16) hipLaunchKernelGGL((column_sums<bf16>), grid, dim3(1024), 0, st, (const bf16*)dy, db, N, out);
+        else hipLaunchKernelGGL((column_sums<float>), grid, dim3(1024), 0, st, (const float*)dy, db, N, out);
+        return hipGetLastError();
+    }
     const int64_t strips = dz_strips(N, out);
     float* part = db ? workspace : nullptr;
     if (is_bf16) launch_dz_t<bf16>(dy, z, dz, part, N, out, act, strips, st);

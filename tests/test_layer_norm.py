@@ -165,6 +165,25 @@ def test_strided_rows(dev, dtype):
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits(dev):
+    """More than 2^31 elements: the last rows' results are those of a call of their own."""
+    from mobilefinetuner_amd import layer_norm as L
+    N, D = (1 << 20) + 300, 2056
+    x = torch.zeros(N, D, dtype=torch.bfloat16, device=dev)
+    last, w, b, dy = (t.to(dev) for t in make(5, D, "bf16", 14))
+    x[-5:] = last
+    y, mean, rstd = L.layer_norm(x, w, b)
+    ref = L.layer_norm(last, w, b)
+    assert torch.equal(y[-5:], ref[0]) and torch.equal(mean[-5:], ref[1]) and torch.equal(rstd[-5:], ref[2])
+    assert torch.equal(y[0], b.bfloat16())
+    y.zero_()  # as dy, but for the last rows
+    y[-5:] = dy
+    dx, dw, _ = L.layer_norm_backward(x, w, mean, rstd, y)
+    assert torch.equal(dx[-5:], L.layer_norm_backward(last, w, *ref[1:], dy)[0]) and (dx[:5] == 0).all()
+    del x, y, dx
+
+
+@pytest.mark.gpu
 def test_values_that_are_not_numbers_stay_in_their_row(dev):
     from mobilefinetuner_amd import layer_norm as L
     x, w, b, dy = (t.to(dev) for t in make(8, 257, "f32", 7))

@@ -143,6 +143,73 @@ def test_large_products(dev, shape, w_t):
         within(db, rb, tb, "db")
 
 
+def within_gpu(got, ref, tol, what):
+    worst = float(((got.double() - ref).abs() / tol).max())
+    assert worst <= 1.0, f"{what}: {worst:.3g} times the bound"
+
+
+# Every tile that a product may run in (256 x 128 and 128 x 128 for two workgroups to a CU, 64 x 64,
+# 256 x 256, and 128, 192 and 256 x 128 for a CU of their own), whole and cut along K, with ragged
+# edges; rows on 16 bytes (multiples of 8) and off them (copied to whole rows first, or read as they
+# are).  W both ways makes each product run with k contiguous in one operand, in both and in none.
+TILES = [(8727, 70, 1178), (518, 5516, 6648), (8554, 196, 864), (5442, 330, 4975), (561, 5634, 5067), (8584, 3457, 616),
+         (8662, 614, 3514), (93, 1856, 2144), (3328, 6573, 67), (64, 1400, 5039), (5693, 144, 5753), (65, 5135, 4161),
+         (1761, 64, 3761), (1020, 66, 5471), (143, 4982, 5773), (6377, 132, 4750), (700, 601, 1203), (1300, 1201, 1501),
+         (8728, 72, 1176), (520, 5512, 6648), (8552, 200, 864), (5440, 328, 4968), (568, 5632, 5064), (8584, 3456, 616),
+         (96, 1864, 2152), (5696, 144, 5752), (64, 5136, 4168), (1768, 72, 3768), (1032, 72, 5480), (144, 4984, 5776)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", TILES, ids=lambda s: "x".join(map(str, s)))
+def test_every_tile(dev, shape):
+    from mobilefinetuner_amd import linear as L
+    N, n_in, n_out = shape
+    g = torch.Generator(device=dev).manual_seed(N)
+
+    def randn(*size):
+        return torch.randn(*size, device=dev, generator=g)
+
+    t = torch.bfloat16
+    x, W = randn(N, n_in).to(t), (randn(n_in, n_out) / math.sqrt(n_in)).to(t)
+    s = dict(x=x, W=W, bias=0.3 * randn(n_out), residual=randn(N, n_out).to(t), dy=(0.1 * randn(N, n_out)).to(t))
+    s["z"] = (x.double() @ W.double() + s["bias"]).to(t)
+    rz, tz, ry, ty = ref_forward(s, "silu", False)
+    rx, tx, rw, tw, rb, tb = ref_backward(s, "silu", False)
+    plain = ref_backward(s, "none", False)
+    for w_t in (False, True):
+        print(f"[case] {shape} {'[out, in]' if w_t else '[in, out]'}", flush=True)
+        w = W.t().contiguous() if w_t else W
+        y, z = L.linear(x, w, s["bias"], "silu", s["residual"], w_t, want_preact=True)
+        within_gpu(y, ry, ty, "y")
+        within_gpu(z, rz, tz, "z")
+        dx, dW, db = L.linear_backward(x, w, s["z"], s["dy"], "silu", w_t)
+        within_gpu(dx, rx, tx, "dx")
+        within_gpu(dW.t() if w_t else dW, rw, tw, "dW")
+        within_gpu(db, rb, tb, "db")
+        dx, dW, db = L.linear_backward(x, w, None, s["dy"], "none", w_t)
+        within_gpu(dx, plain[0], plain[1], "dx")
+        within_gpu(dW.t() if w_t else dW, plain[2], plain[3], "dW")
+        within_gpu(db, plain[4], plain[5], "db")
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(dev):
+    """y with more than 2^31 elements: its first and last rows are those of a call of their own
+    (a row's terms are added in the same order in every tile but the groups' of a CU's own, whose
+    two sums are added last: 2 (K + 8) u of the magnitudes, and the rounding of each)."""
+    from mobilefinetuner_amd import linear as L
+    N, n_in, n_out = (1 << 19) + 40, 64, 4160
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.randn(N, n_in, device=dev, generator=g).bfloat16()
+    W = (torch.randn(n_in, n_out, device=dev, generator=g) / 8).bfloat16()
+    y = L.linear(x, W)[0]
+    for rows in (slice(0, 300), slice(N - 300, N)):
+        s = dict(x=x[rows], W=W, bias=None)
+        _, _, ry, ty = ref_forward(s, "none", False, False, False)
+        within_gpu(y[rows], ry, ty, "y")
+    del y
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("N", [1, 40])
