@@ -28,6 +28,11 @@ struct GemmF32 {
     const float* bias;  // [N] or null
     int add;
     float* partial;     // workspace of gemm_f32_workspace bytes (may be null where that is 0)
+    // The linear layer's epilogue, with ldc = N, A stored [M, K] and no add: z (null: not kept) is
+    // the sum with its bias, C = act(z) + residual (null: none), an ACT_* of linear_kernels.h.
+    int act;
+    const float* residual;
+    float* z;
 };
 
 // Workspace bytes: fp32 partial products where K is split across workgroups.

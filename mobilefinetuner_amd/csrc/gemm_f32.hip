@@ -54,6 +54,7 @@
 #include "attn_common.h"
 #include "attn_geometry.h"
 #include "attn_kernels.h"
+#include "linear_epilogue.h"
 #include "prologue_kernels.h"
 
 namespace mft {
@@ -185,9 +186,25 @@ struct Doubt {
     __device__ __forceinline__ bool any() const { return least < ((127u - 80u) << 24) - 1u || sum != sum; }
 };
 
-// TA / TB: term 0's storage.  KW groups of 2 x 2 waves share a stage's 16-deep
+// The linear layer's epilogue of VEC columns n of row m (GemmF32).
+template <int VEC> __device__ __forceinline__ void run_epilogue(const GemmF32& g, int64_t m, int64_t n, float* v) {
+    LinearProduct p{};
+    p.N = g.N;
+    p.C = g.C;
+    p.bias = g.bias;
+    p.residual = g.residual;
+    p.z = g.z;
+    switch (g.act) {
+        case ACT_RELU: linear_epilogue<float, ACT_RELU, VEC>(p, m, n, v); break;
+        case ACT_GELU_TANH: linear_epilogue<float, ACT_GELU_TANH, VEC>(p, m, n, v); break;
+        case ACT_SILU: linear_epilogue<float, ACT_SILU, VEC>(p, m, n, v); break;
+        default: linear_epilogue<float, ACT_NONE, VEC>(p, m, n, v); break;
+    }
+}
+
+// TA / TB: term 0's storage.  EPI: with the linear layer's epilogue.  KW groups of 2 x 2 waves share a stage's 16-deep
 // k steps; their accumulators are added through LDS at the end.
-template <int T, int BK, int KW, bool TA, bool TB>
+template <int T, int BK, int KW, bool TA, bool TB, bool EPI>
 __global__ __launch_bounds__(256 * KW, 3) void gemm_f32_kernel(Args a) {
     constexpr int MT = T / 64, NT = T / 64;  // 32 x 32 tiles per wave
     constexpr int kThreads = 256 * KW, KS = BK / 16 / KW;  // k steps of a wave per stage
@@ -486,6 +503,13 @@ __global__ __launch_bounds__(256 * KW, 3) void gemm_f32_kernel(Args a) {
             for (int q = 0; q < 4; ++q) {
                 const int64_t c0 = nw + 32 * j + 8 * q;
                 f32x4 o{acc[j][k][4 * q], acc[j][k][4 * q + 1], acc[j][k][4 * q + 2], acc[j][k][4 * q + 3]};
+                if constexpr (EPI) {
+                    if (a.whole) {
+                        float v[4] = {o[0], o[1], o[2], o[3]};
+                        if (c0 < a.g.N) run_epilogue<4>(a.g, m, c0, v);
+                        continue;
+                    }
+                }
                 float* d = C + m * ldc + c0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -501,8 +525,8 @@ __global__ __launch_bounds__(256 * KW, 3) void gemm_f32_kernel(Args a) {
     }
 }
 
-// C (+)= the slices' partial products in slice order, + bias.
-template <int VEC>
+// C (+)= the slices' partial products in slice order, + bias (EPI: and the linear layer's epilogue).
+template <int VEC, bool EPI>
 __global__ __launch_bounds__(256) void gemm_f32_reduce(Args a) {
     typedef float V __attribute__((ext_vector_type(VEC)));
     const int64_t MN = a.g.M * a.g.N, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
@@ -511,6 +535,13 @@ __global__ __launch_bounds__(256) void gemm_f32_reduce(Args a) {
     V sum = *reinterpret_cast<const V*>(a.g.partial + i);
 #pragma unroll 8
     for (int s = 1; s < a.slices; ++s) sum += *reinterpret_cast<const V*>(a.g.partial + s * MN + i);
+    if constexpr (EPI) {
+        float v[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = sum[e];
+        run_epilogue<VEC>(a.g, m, n, v);
+        return;
+    }
     float* d = a.g.C + m * a.g.ldc + n;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) d[e] = sum[e] + (a.g.bias ? a.g.bias[n + e] : 0.f) + (a.g.add ? d[e] : 0.f);
@@ -559,18 +590,31 @@ Plan plan(const GemmF32& g) {
     return p;
 }
 
+bool with_epilogue(const GemmF32& g) { return g.act != ACT_NONE || g.residual || g.z; }
+
 template <int T, int BK, int KW>
 void launch_t(const Args& a, hipStream_t st) {
     const dim3 grid((unsigned)(a.tiles_m * a.tiles_n * a.slices));
     const bool ta = a.g.terms[0].ta != 0, tb = a.g.terms[0].tb != 0;
-    if (ta && tb)
-        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, true, true>), grid, dim3(256 * KW), 0, st, a);
+    if (with_epilogue(a.g)) {
+        if (tb)
+            hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, true, true>), grid, dim3(256 * KW), 0, st, a);
+        else
+            hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, false, true>), grid, dim3(256 * KW), 0, st, a);
+    } else if (ta && tb)
+        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, true, true, false>), grid, dim3(256 * KW), 0, st, a);
     else if (ta)
-        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, true, false>), grid, dim3(256 * KW), 0, st, a);
+        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, true, false, false>), grid, dim3(256 * KW), 0, st, a);
     else if (tb)
-        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, true>), grid, dim3(256 * KW), 0, st, a);
+        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, true, false>), grid, dim3(256 * KW), 0, st, a);
     else
-        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, false>), grid, dim3(256 * KW), 0, st, a);
+        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, false, false>), grid, dim3(256 * KW), 0, st, a);
+}
+
+template <int VEC> void launch_reduce(const Args& a, hipStream_t st) {
+    const dim3 grid((unsigned)((a.g.M * a.g.N / VEC + 255) / 256));
+    if (with_epilogue(a.g)) hipLaunchKernelGGL((gemm_f32_reduce<VEC, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((gemm_f32_reduce<VEC, false>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -582,6 +626,7 @@ size_t gemm_f32_workspace(const GemmF32& g) {
 
 hipError_t launch_gemm_f32(const GemmF32& g, hipStream_t st) {
     if (g.M <= 0 || g.N <= 0) return hipSuccess;
+    if (with_epilogue(g) && (g.ldc != g.N || g.terms[0].ta || g.add)) return hipErrorInvalidValue;
     const Plan p = plan(g);
     if (p.small)
         launch_t<64, 32, 2>(p.a, st);
@@ -589,11 +634,8 @@ hipError_t launch_gemm_f32(const GemmF32& g, hipStream_t st) {
         launch_t<128, 16, 1>(p.a, st);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.a.whole) return e;
-    const int64_t MN = g.M * g.N;
-    if (g.N % 4 == 0)
-        hipLaunchKernelGGL(gemm_f32_reduce<4>, dim3((unsigned)((MN / 4 + 255) / 256)), dim3(256), 0, st, p.a);
-    else
-        hipLaunchKernelGGL(gemm_f32_reduce<1>, dim3((unsigned)((MN + 255) / 256)), dim3(256), 0, st, p.a);
+    if (g.N % 4 == 0) launch_reduce<4>(p.a, st);
+    else launch_reduce<1>(p.a, st);
     return hipGetLastError();
 }
 

@@ -358,7 +358,7 @@ struct Shape {
 };
 Shape fwd_shape(int64_t D, int vec) {
     for (const Shape s : {Shape{1, 1}, {1, 2}, {1, 4}, {1, 8}, {4, 4}, {4, 8}, {16, 4}, {16, 8}})
-        if (D <= (int64_t)64 * s.wpr * s.ch * vec) return s;
+        if (D <= (int64_t)64 * s.wpr * s.ch * vec && s.ch * vec * s.wpr <= 512) return s;  // 16 waves: 128 registers
     return {0, 0};
 }
 Shape bwd_shape(int64_t D, int vec) {

@@ -1,6 +1,6 @@
-// Element-wise passes of the linear layer (C ABI in include/mft/linear.h): the
-// activation over fp32 products, and the backward's dz = dy act'(z) with the
-// bias gradient's column sums.  Bound by memory.
+// Element-wise passes of the linear layer's backward (C ABI in
+// include/mft/linear.h): dz = dy act'(z) and the bias gradient, its column sums.
+// Bound by memory.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -11,19 +11,6 @@
 
 namespace mft {
 namespace {
-
-template <int ACT>
-__global__ __launch_bounds__(256) void act_kernel(const float* z, const float* residual, float* y, int64_t n) {
-    const int64_t step = (int64_t)gridDim.x * 256 * 4;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += step) {
-        float v[4], r[4];
-        load_part<float, 4>(z, i, n, v);
-        if (residual) load_part<float, 4>(residual, i, n, r);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = act_value<ACT>(v[e]) + (residual ? r[e] : 0.f);
-        store_part<float, 4>(y, i, n, v);
-    }
-}
 
 // A workgroup takes 64 threads' columns (V each) and every strips-th row group:
 // its four waves the rows in turn.
@@ -124,20 +111,6 @@ void launch_dz_t(const void* dy, const void* z, void* dz, float* part, int64_t N
 }
 
 }  // namespace
-
-hipError_t launch_act(const float* z, const float* residual, float* y, int64_t n, int act, hipStream_t st) {
-    if (n == 0) return hipSuccess;
-    const dim3 grid((unsigned)std::min<int64_t>((n + 1023) / 1024, 8 * device_cus()));
-#define MFT_ACT(ACT) hipLaunchKernelGGL((act_kernel<ACT>), grid, dim3(256), 0, st, z, residual, y, n)
-    switch (act) {
-        case ACT_RELU: MFT_ACT(ACT_RELU); break;
-        case ACT_GELU_TANH: MFT_ACT(ACT_GELU_TANH); break;
-        case ACT_SILU: MFT_ACT(ACT_SILU); break;
-        default: MFT_ACT(ACT_NONE); break;
-    }
-#undef MFT_ACT
-    return hipGetLastError();
-}
 
 size_t dz_workspace(int64_t N, int64_t out) { return (size_t)dz_strips(N, out) * out * 4; }
 

@@ -151,25 +151,10 @@ mft_status mft_linear_fwd(const mft_linear_desc* desc, const void* x, const void
     }
     mft::GemmF32 g = f_fwd(desc);
     g.bias = bias;
-    if (desc->activation == MFT_ACT_NONE) {
-        if (residual == y) {
-            g.add = 1;
-            return hip_status(run_f32(g, x, W, y, ws, stream), "mft_linear_fwd launch");
-        }
-        hipError_t e = run_f32(g, x, W, y, ws, stream);
-        if (e == hipSuccess && residual)
-            e = mft::launch_act(static_cast<const float*>(y), static_cast<const float*>(residual),
-                                static_cast<float*>(y), desc->N * desc->out_dim, desc->activation, stream);
-        return hip_status(e, "mft_linear_fwd launch");
-    }
-    if (!z && residual == y)
-        return fail(MFT_ERR_UNSUPPORTED, "mft_linear_fwd: fp32 with an activation and residual == y needs z");
-    void* to = z ? z : y;
-    hipError_t e = run_f32(g, x, W, to, ws, stream);
-    if (e == hipSuccess)
-        e = mft::launch_act(static_cast<const float*>(to), static_cast<const float*>(residual), static_cast<float*>(y),
-                            desc->N * desc->out_dim, desc->activation, stream);
-    return hip_status(e, "mft_linear_fwd launch");
+    g.act = desc->activation;
+    g.residual = static_cast<const float*>(residual);
+    g.z = static_cast<float*>(z);
+    return hip_status(run_f32(g, x, W, y, ws, stream), "mft_linear_fwd launch");
 }
 
 mft_status mft_linear_bwd(const mft_linear_desc* desc, const void* x, const void* W, const void* z, const void* dy,

@@ -35,9 +35,6 @@ hipError_t launch_bf_gemm(const LinearProduct& g, hipStream_t st);
 bool few_rows(const LinearProduct& g);
 hipError_t launch_few_rows(const LinearProduct& g, bool bf16, hipStream_t st);
 
-// y = act(z) + residual over n values; y may be z or residual.
-hipError_t launch_act(const float* z, const float* residual, float* y, int64_t n, int act, hipStream_t st);
-
 // dz = dy act'(z) ([N, out]; no act: dz is not written) and db[out] = the sums
 // of dz's columns before rounding (null: left out).
 size_t dz_workspace(int64_t N, int64_t out);

@@ -233,6 +233,26 @@ def test_parts_of_the_epilogue_and_of_the_gradient(dev, dtype, N):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 96, 80), (40, 96, 80), (64, 4096, 72), (300, 65, 131)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_residual_in_place(dev, dtype, shape):
+    """y given the residual's own memory, through the C ABI: one row, a tile, K cut into slices, odd sizes."""
+    from mobilefinetuner_amd import capi, linear as L
+    N, n_in, n_out = shape
+    d = {k: v.to(dev) for k, v in make(*shape, dtype, 11).items()}
+    for act in ("none", "silu"):
+        ref = L.linear(d["x"], d["W"], d["bias"], act, d["residual"])[0]
+        y = d["residual"].clone()
+        desc = capi.linear_desc(N, n_in, n_out, capi.MFT_BF16 if dtype == "bf16" else capi.MFT_F32, False,
+                                L.ACTIVATIONS[act])
+        ws = torch.empty(max(1, capi.linear_workspace_size(desc)[0]), dtype=torch.uint8, device=dev)
+        capi.linear_fwd(desc, d["x"].data_ptr(), d["W"].data_ptr(), d["bias"].data_ptr(), y.data_ptr(), y.data_ptr(),
+                        None, ws.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(y, ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_no_rows_and_leading_dimensions(dev, dtype):
     from mobilefinetuner_amd import linear as L
     d = {k: v.to(dev) for k, v in make(6, 40, 24, dtype, 5).items()}
