@@ -18,8 +18,8 @@
  * bf16, dz is rounded to bf16 for the matrix units where there is an activation
  * (half a step of each product's operand, as x and W have; dbias is summed
  * before that), dx and dW once more where they are stored.  With fp32 the
- * products are those of the LoRA layer's (csrc/gemm_f32.hip).  Results do not
- * depend on the order in which workgroups run.
+ * products are those of the LoRA layer's (csrc/gemm_f32.hip), and with one or two
+ * rows fp32 sums.  Results do not depend on the order in which workgroups run.
  *
  * Conventions are those of mft/attention.h (status codes, mft_last_error,
  * caller-owned device memory, stream ordering, no allocation).  All operands

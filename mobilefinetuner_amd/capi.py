@@ -396,6 +396,13 @@ def linear_workspace_size(d):
     return f.value, b.value
 
 
+def linear_fwd_workspace_size(d) -> int:
+    """The forward's alone: a call for its products need not plan the backward's."""
+    f = C.c_size_t()
+    check(lib().mft_linear_workspace_size(C.byref(d), C.byref(f), None))
+    return f.value
+
+
 def linear_fwd(d, x, W, bias, residual, y, z, workspace, stream) -> None:
     check(lib().mft_linear_fwd(C.byref(d), x, W, bias, residual, y, z, workspace, stream))
 

@@ -42,7 +42,6 @@ namespace mft {
 namespace {
 
 constexpr int kThreads = 256;
-
 constexpr int kHalf = 32, kSlab = 64;  // k of a pipeline step, and of a slab with k contiguous
 
 struct Args {
@@ -53,7 +52,8 @@ struct Args {
     FastDiv per_slice_tiles;
 };
 
-__device__ __forceinline__ constexpr int swz_kc(int r) { return (r >> 1) & 7; }  // 16 rows' reads of a chunk: 16 banks' groups
+// 16 rows' reads of one chunk of a slab of 64 meet no bank twice.
+__device__ __forceinline__ constexpr int swz_kc(int r) { return (r >> 1) & 7; }
 
 // One operand of R rows a tile, for a workgroup of W waves: RING slabs of SK k.
 template <int R, bool KC, int W = 4, int SK = KC ? kSlab : kHalf, int RING = KC ? 2 : 3> struct Operand {
@@ -79,8 +79,8 @@ template <int R, bool KC, int W = 4, int SK = KC ? kSlab : kHalf, int RING = KC 
                 const int r = (w * PER + j) * (64 / CPR) + lane / CPR, c = lane % CPR ^ swz_of(r);
                 if (KC)  // rows past the end are read again from the last one, and not stored
                     off[j] = (uint32_t)((min(r0 + r, rows - 1) - r0) * ld * 2) + 16u * c;
-                else
-                    off[j] = (uint32_t)(r * ld * 2) + (uint32_t)(min(r0 + 8 * c, (rows - 1) / 8 * 8) - r0) * 2u;  // rows are of whole chunks
+                else  // whole chunks, the last of them again past the end
+                    off[j] = (uint32_t)(r * ld * 2) + (uint32_t)(min(r0 + 8 * c, (rows - 1) / 8 * 8) - r0) * 2u;
             }
         }
         // Load j of the slab whose first element is `from`, into the slab at LDS address `to`.
@@ -147,7 +147,6 @@ template <int R, bool KC, int T> struct Fragments {
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
-    static constexpr int kReads = KC ? T : 2 * T;
 };
 
 // This workgroup's slice and tile.
@@ -203,7 +202,7 @@ __global__ __launch_bounds__(kThreads, BN * BM > 32768 ? 1 : 2) void bf_gemm_ker
     constexpr int kStaged = 4 * 32 * kPitch * 4, kSlabs = OpQ::kBytes + OpP::kBytes;
     __shared__ __attribute__((aligned(1024))) char smem[kSlabs > kStaged ? kSlabs : kStaged];  // [Q slabs][P slabs]
     char* const lds_p = smem + OpQ::kBytes;
-    const int lane = threadIdx.x & 63, w = wave_id(), hh = lane >> 5;
+    const int lane = threadIdx.x & 63, w = wave_id();
     const int wn = w & 1, wm = w >> 1;
 
     int slice;
@@ -302,8 +301,8 @@ __global__ __launch_bounds__(kThreads, BN * BM > 32768 ? 1 : 2) void bf_gemm_ker
                 for (int j = 0; j < n; ++j)
                     if (j >= from + t * count / kTiles && j < from + (t + 1) * count / kTiles) issue_one(h, odd_t, j);
             };
-            // One half, ODD its place in its pair; LEFT: halves after it (4: at least four).  The loads of
-            // half h + 3 go out behind the barrier, when half h's slabs are free, and in half h + 1.
+            // One half, ODD its place in its pair; LEFT: halves after it (3: at least three).  The
+            // loads of half h + 3 go out behind the barrier, when half h's slabs are free, and in half h + 1.
             auto half = [&](int h, auto odd_t, auto left_t) {
                 constexpr bool ODD = decltype(odd_t)::value;
                 constexpr int LEFT = decltype(left_t)::value;
@@ -377,7 +376,7 @@ __global__ __launch_bounds__(kThreads, BN * BM > 32768 ? 1 : 2) void bf_gemm_ker
         }
     }
 
-    lds_barrier();
+    lds_barrier();  // the slabs have been read
     float* st = reinterpret_cast<float*>(smem) + w * 32 * kPitch;
 #pragma unroll
     for (int k = 0; k < TM; ++k) {

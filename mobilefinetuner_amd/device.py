@@ -41,17 +41,17 @@ def ptr(t):
 
 
 def operand(t, name, like=None, dtype=None, shape=None):
-    """t, checked: on the GPU (`like`'s, if given), of `dtype` and `shape` where they are given."""
+    """t, checked: on the GPU (`like`'s, if given), of `dtype` and `shape` (a tuple) where they are given."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor (there is no CPU path)")
-    if like is not None and t.device != like.device:
+    if like is not None and t.get_device() != like.get_device():
         raise ValueError(f"{name} is on {t.device}, the call on {like.device}")
     if dtype is None:
         if t.dtype not in DTYPES:
             raise ValueError(f"{name}: unsupported dtype {t.dtype}")
     elif t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     return t
 
@@ -65,7 +65,7 @@ def rows(t, last):
     """t [..., last] as [N, last] with one stride between rows: a view where its
     strides allow, else a copy."""
     if t.dim() != 2:
-        t = t.reshape(-1, last)
+        t = t.view(-1, last) if t.is_contiguous() else t.reshape(-1, last)
     if t.stride(1) == 1 or last == 1:
         if t.stride(0) >= last:
             return t

@@ -50,7 +50,7 @@ def linear(x, W, bias=None, activation="none", residual=None, w_transposed=False
         xc, Wc = x.contiguous(), W.contiguous()
         y = torch.empty(*lead, n_out, dtype=x.dtype, device=x.device)
         z = torch.empty_like(y) if want_preact else None
-        ws = workspace(capi.linear_workspace_size(d)[0], x)
+        ws = workspace(capi.linear_fwd_workspace_size(d), x)
         capi.linear_fwd(d, xc.data_ptr(), Wc.data_ptr(), ptr(bias), ptr(residual), y.data_ptr(), ptr(z), ptr(ws),
                         stream(x))
     return y, z

@@ -66,11 +66,11 @@ def token_logprobs_backward(logits, tokens, stats, entropy, grad_logprob, grad_e
 
 
 class TokenLogprobs(torch.autograd.Function):
-    """logprob, entropy = TokenLogprobs.apply(logits, tokens, ignore_index)."""
+    """logprob, entropy = TokenLogprobs.apply(logits, tokens, ignore_index, check_tokens)."""
 
     @staticmethod
-    def forward(ctx, logits, tokens, ignore_index=-100):
-        logprob, entropy, stats, _, _ = token_logprobs(logits, tokens, 0, ignore_index)
+    def forward(ctx, logits, tokens, ignore_index=-100, check_tokens=True):
+        logprob, entropy, stats, _, _ = token_logprobs(logits, tokens, 0, ignore_index, check_tokens)
         ctx.save_for_backward(logits, tokens, stats, entropy)
         ctx.ignore_index = ignore_index
         ctx.set_materialize_grads(False)
@@ -79,7 +79,7 @@ class TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_logprob, grad_entropy):
         if grad_logprob is None and grad_entropy is None:
-            return None, None, None
+            return None, None, None, None
         logits, tokens, stats, entropy = ctx.saved_tensors
         return token_logprobs_backward(logits, tokens, stats, entropy, grad_logprob, grad_entropy,
-                                       ctx.ignore_index), None, None
+                                       ctx.ignore_index), None, None, None
