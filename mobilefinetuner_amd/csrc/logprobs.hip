@@ -31,7 +31,10 @@ namespace mft {
 namespace {
 
 constexpr int kLpThreads = 256, kLpWaves = kLpThreads / 64;
-constexpr int kUnroll = 4;  // vectors in flight per thread
+// Vectors in flight per thread: 2048 rows of 50257 in fp32 with five alternatives 91
+// us with 2, 89 with 4, 82 with 8 (5.0 TB/s).
+constexpr int kUnroll = 8;
+constexpr int kBwdVecs = 4;  // of a thread of the backward's workgroups
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
 constexpr float kLowest = -1e30f;  // in place of -inf in a product with a probability of 0
 
@@ -410,7 +413,7 @@ hipError_t launch_logprobs_fwd(LogprobsArgs a, bool is_bf16, void* workspace, hi
 hipError_t launch_logprobs_bwd(const LogprobsArgs& args, bool is_bf16, hipStream_t st) {
     if (args.N == 0) return hipSuccess;
     LogprobsArgs a = args;
-    a.per_part = (int64_t)kLpThreads * kUnroll * (is_bf16 ? kVec<bf16> : kVec<float>);
+    a.per_part = (int64_t)kLpThreads * kBwdVecs * (is_bf16 ? kVec<bf16> : kVec<float>);
     // the grid stays within 2^31 - 1 workgroups
     while (a.N * ((a.V + a.per_part - 1) / a.per_part) > (int64_t(1) << 31) - 1) a.per_part *= 2;
     a.parts = (int)((a.V + a.per_part - 1) / a.per_part);
