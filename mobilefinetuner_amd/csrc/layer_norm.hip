@@ -3,8 +3,10 @@
 //
 // A row is held in registers, by one wave (WPR = 1), four or sixteen: one read
 // of x, the mean, then the sums of d = x - mean and d^2 about it, so that a
-// mean far above the deviation costs no digits (the sum of d, which is zero but
-// for the mean's rounding, corrects the mean by the part it was rounded by).
+// mean far above the deviation costs no digits: there d is exact, and its sum,
+// zero but for the mean's rounding, corrects the mean.  A mean below the deviation
+// is taken as it is: x - mean then rounds alike for all x of one binade, and the
+// sum of d would carry that (mean of 8192 normal values: 8e-7 off with it).
 // Longer rows are read once per sum.  All of it is bound by memory.
 //
 // Backward: the row sums of g = dy w and g h give dx in one pass over x and dy.
@@ -60,24 +62,26 @@ __global__ __launch_bounds__(kThreads<WPR>) void ln_fwd(LayerNormArgs a) {
     float sum = 0.f, none = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) load_part<T, V>(xr, (int64_t)(c * TPR + t) * V, a.D, x[c]);
+    // Sums of a vector in pairs: a mean near zero is a small difference of its addends.
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int e = 0; e < V; ++e) sum += x[c][e];
+    for (int c = 0; c < CH; ++c) sum += sum_pairs<V>(x[c]);
     row_sum2<WPR>(sum, none, s1);
     const float inv = 1.0f / (float)a.D;
     float mean = sum * inv, d1 = 0.f, d2 = 0.f;
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < CH; ++c) {
+        float q[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const float d = (int64_t)(c * TPR + t) * V + e < a.D ? x[c][e] - mean : 0.f;
             x[c][e] = d;
-            d1 += d;
-            d2 = fmaf(d, d, d2);
+            q[e] = d * d;
         }
+        d1 += sum_pairs<V>(x[c]);
+        d2 += sum_pairs<V>(q);
+    }
     row_sum2<WPR>(d1, d2, s2);
-    const float off = d1 * inv;  // what the mean's rounding left
+    const float off = mean * mean <= d2 * inv ? 0.f : d1 * inv;  // what the mean's rounding left; NaN stays
     const float rstd = 1.0f / sqrtf(fmaxf(fmaf(-off, off, d2 * inv), 0.f) + a.eps);
     T* yr = (T*)a.y + n * a.sy;
 #pragma unroll
@@ -111,29 +115,26 @@ template <typename T> __global__ __launch_bounds__(kLongThreads) void ln_fwd_lon
     const float inv = 1.0f / (float)a.D;
     float sum = 0.f, none = 0.f;
     for (int64_t d0 = (int64_t)threadIdx.x * V; d0 < a.D; d0 += kLongThreads * V) {
-        float x[V], p = 0.f;
+        float x[V];
         load_part<T, V>(xr, d0, a.D, x);
-#pragma unroll
-        for (int e = 0; e < V; ++e) p += x[e];
-        sum += p;
+        sum += sum_pairs<V>(x);
     }
     row_sum2<kLongWaves>(sum, none, s1);
     const float mean = sum * inv;
     float d1 = 0.f, d2 = 0.f;
     for (int64_t d0 = (int64_t)threadIdx.x * V; d0 < a.D; d0 += kLongThreads * V) {
-        float x[V], p1 = 0.f, p2 = 0.f;
+        float x[V], q[V];
         load_part<T, V>(xr, d0, a.D, x);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float d = d0 + e < a.D ? x[e] - mean : 0.f;
-            p1 += d;
-            p2 = fmaf(d, d, p2);
+            x[e] = d0 + e < a.D ? x[e] - mean : 0.f;
+            q[e] = x[e] * x[e];
         }
-        d1 += p1;
-        d2 += p2;
+        d1 += sum_pairs<V>(x);
+        d2 += sum_pairs<V>(q);
     }
     row_sum2<kLongWaves>(d1, d2, s2);
-    const float off = d1 * inv;
+    const float off = mean * mean <= d2 * inv ? 0.f : d1 * inv;
     const float rstd = 1.0f / sqrtf(fmaxf(fmaf(-off, off, d2 * inv), 0.f) + a.eps);
     T* yr = (T*)a.y + n * a.sy;
     for (int64_t d0 = (int64_t)threadIdx.x * V; d0 < a.D; d0 += kLongThreads * V) {
@@ -387,7 +388,7 @@ template <typename T> hipError_t fwd(const LayerNormArgs& a, hipStream_t st) {
     MFT_LN_FWD(4, 4);
     MFT_LN_FWD(4, 8);
     MFT_LN_FWD(16, 4);
-    MFT_LN_FWD(16, 8);
+    if constexpr (kVec<T> == 4) MFT_LN_FWD(16, 8);
 #undef MFT_LN_FWD
     if (s.wpr == 0) hipLaunchKernelGGL((ln_fwd_long<T>), grid, dim3(kLongThreads), 0, st, a);
     return hipGetLastError();

@@ -49,6 +49,12 @@ __device__ __forceinline__ void store_part(T* row, int64_t d0, int64_t D, const 
     }
 }
 
+// Sum of V values (a power of two) in pairs.
+template <int V> __device__ __forceinline__ float sum_pairs(const float* x) {
+    if constexpr (V == 1) return x[0];
+    else return sum_pairs<V / 2>(x) + sum_pairs<V / 2>(x + V / 2);
+}
+
 template <int CTRL> __device__ __forceinline__ float dpp(float x) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
 }

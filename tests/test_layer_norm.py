@@ -3,8 +3,9 @@
 
 Bounds, per element, with u = 2^-24 and K = 80 (the longest chain of fp32
 additions of a row's sum: 64 values of a thread, then the tree over threads).
-The mean is corrected by the sum about it, so its error is K u of the mean
-deviation, which rstd scales to at most 1; rstd's relative error is half of its
+A mean above the deviation is corrected by the sum about it, so its error is K u
+of the mean deviation, which rstd scales to at most 1; one below has K u of the
+mean magnitude, at most sqrt(2) deviations.  rstd's relative error is half of its
 sum's and a few roundings.  So h = (x - mean) rstd is off by
 u ((K / 2 + 8) |h| + 2 K), and y by |w| times that, the roundings of the
 product and the sum, and half a step of its type.  The backward takes the
