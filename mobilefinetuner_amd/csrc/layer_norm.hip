@@ -376,8 +376,13 @@ int64_t bwd_groups(int64_t N, int64_t D, int vec) {
 }
 size_t up(size_t x) { return (x + 255) & ~size_t(255); }
 
-template <typename T> hipError_t fwd(const LayerNormArgs& a, hipStream_t st) {
-    const Shape s = fwd_shape(a.D, kVec<T>);
+// f(first row, rows) for as many rows at a time as a launch's 2^32 threads allow.
+template <typename F> void row_slices(int64_t N, int wpr, F f) {
+    const int64_t most = (int64_t(1) << 31) / (64 * (wpr ? wpr : kLongWaves));
+    for (int64_t n = 0; n < N; n += most) f(n, std::min(most, N - n));
+}
+
+template <typename T> void fwd_rows(const LayerNormArgs& a, const Shape& s, hipStream_t st) {
     const dim3 grid((unsigned)(s.wpr == 1 ? (a.N + 3) / 4 : a.N));
 #define MFT_LN_FWD(WPR, CH) \
     if (s.wpr == WPR && s.ch == CH) hipLaunchKernelGGL((ln_fwd<T, WPR, CH>), grid, dim3(kThreads<WPR>), 0, st, a)
@@ -391,6 +396,18 @@ template <typename T> hipError_t fwd(const LayerNormArgs& a, hipStream_t st) {
     if constexpr (kVec<T> == 4) MFT_LN_FWD(16, 8);
 #undef MFT_LN_FWD
     if (s.wpr == 0) hipLaunchKernelGGL((ln_fwd_long<T>), grid, dim3(kLongThreads), 0, st, a);
+}
+template <typename T> hipError_t fwd(const LayerNormArgs& a, hipStream_t st) {
+    const Shape s = fwd_shape(a.D, kVec<T>);
+    row_slices(a.N, s.wpr, [&](int64_t n, int64_t rows) {
+        LayerNormArgs q = a;
+        q.N = rows;
+        q.x = (const T*)a.x + n * a.sx;
+        q.y = (T*)a.y + n * a.sy;
+        if (a.mean) q.mean = a.mean + n;
+        if (a.rstd) q.rstd = a.rstd + n;
+        fwd_rows<T>(q, s, st);
+    });
     return hipGetLastError();
 }
 
@@ -401,7 +418,15 @@ template <typename T> hipError_t bwd(const LayerNormArgs& a, hipStream_t st) {
         LayerNormArgs q = a;
         if (!params) q.part = nullptr;
         if (a.dx) {
-            hipLaunchKernelGGL((ln_bwd_sums<T>), dim3((unsigned)a.N), dim3(kLongThreads), 0, st, q);
+            row_slices(a.N, 0, [&](int64_t n, int64_t rows) {
+                LayerNormArgs r = a;
+                r.x = (const T*)a.x + n * a.sx;
+                r.dy = (const T*)a.dy + n * a.sdy;
+                r.mean_in = a.mean_in + n;
+                r.rstd_in = a.rstd_in + n;
+                r.sums = a.sums + n;
+                hipLaunchKernelGGL((ln_bwd_sums<T>), dim3((unsigned)rows), dim3(kLongThreads), 0, st, r);
+            });
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
         }

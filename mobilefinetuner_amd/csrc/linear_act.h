@@ -12,7 +12,7 @@ constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluA = 0.044715f;
 
 template <int ACT> __device__ __forceinline__ float act_value(float z) {
-    if constexpr (ACT == ACT_RELU) return z > 0.f ? z : z * 0.f;  // a NaN stays
+    if constexpr (ACT == ACT_RELU) return z <= 0.f ? 0.f : z;  // a NaN stays
     if constexpr (ACT == ACT_GELU_TANH || ACT == ACT_SILU) {
         // exponent of 2 of exp(-2 u), or of exp(-z)
         const float x = ACT == ACT_SILU ? z * -kLog2e

@@ -29,9 +29,9 @@ mft_status check(const mft_linear_desc* d, const char* who) {
         return fail(MFT_ERR_INVALID_ARG, std::string(who) + ": dtype must be MFT_F32 or MFT_BF16");
     if (d->activation < MFT_ACT_NONE || d->activation > MFT_ACT_SILU)
         return fail(MFT_ERR_INVALID_ARG, std::string(who) + ": activation must be NONE, RELU, GELU_TANH or SILU");
-    // a tile grid of the products stays within a launch's limit
+    // a launch takes fewer than 2^32 threads: 2^23 tiles of at most 256
     const int64_t n = (d->N + 63) / 64, i = (d->in_dim + 63) / 64, o = (d->out_dim + 63) / 64;
-    if (std::max(n * o, std::max(n * i, i * o)) > (int64_t(1) << 25))
+    if (std::max(n * o, std::max(n * i, i * o)) > (int64_t(1) << 23))
         return fail(MFT_ERR_UNSUPPORTED, std::string(who) + ": N, in and out are too large together");
     return MFT_OK;
 }

@@ -414,8 +414,8 @@ hipError_t launch_logprobs_bwd(const LogprobsArgs& args, bool is_bf16, hipStream
     if (args.N == 0) return hipSuccess;
     LogprobsArgs a = args;
     a.per_part = (int64_t)kLpThreads * kBwdVecs * (is_bf16 ? kVec<bf16> : kVec<float>);
-    // the grid stays within 2^31 - 1 workgroups
-    while (a.N * ((a.V + a.per_part - 1) / a.per_part) > (int64_t(1) << 31) - 1) a.per_part *= 2;
+    // a launch takes fewer than 2^32 threads
+    while (a.N * ((a.V + a.per_part - 1) / a.per_part) >= (int64_t(1) << 32) / kLpThreads) a.per_part *= 2;
     a.parts = (int)((a.V + a.per_part - 1) / a.per_part);
     const dim3 grid((unsigned)(a.N * a.parts));
     if (is_bf16) hipLaunchKernelGGL((lp_bwd<bf16>), grid, dim3(kLpThreads), 0, st, a);

@@ -17,8 +17,8 @@ mft_status check(const mft_logprobs_desc* d, const char* who, mft::LogprobsArgs*
     if (!d) return fail(MFT_ERR_INVALID_ARG, std::string(who) + ": desc is NULL");
     if (d->N < 0 || d->V <= 0)
         return fail(MFT_ERR_INVALID_ARG, std::string(who) + ": logits must be [N, V] with N >= 0 and V > 0");
-    if (d->N > (int64_t(1) << 24) || d->V > (int64_t(1) << 30))
-        return fail(MFT_ERR_UNSUPPORTED, std::string(who) + ": N must be at most 2^24 and V at most 2^30");
+    if (d->N >= (int64_t(1) << 24) || d->V > (int64_t(1) << 30))
+        return fail(MFT_ERR_UNSUPPORTED, std::string(who) + ": N must be below 2^24 and V at most 2^30");
     if (d->dtype != MFT_F32 && d->dtype != MFT_BF16)
         return fail(MFT_ERR_INVALID_ARG, std::string(who) + ": dtype must be MFT_F32 or MFT_BF16");
     if (d->top < 0 || d->top > std::min<int64_t>(d->V, MFT_LOGPROBS_MAX_TOP))

@@ -185,6 +185,27 @@ def test_offsets_past_32_bits(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N,D", [((1 << 25) + 70, 8), ((1 << 21) + 3, 16400)])
+def test_more_rows_than_a_launch_takes(dev, N, D):
+    """Rows held by a wave, by sixteen, and their last ones as in a call of their own."""
+    from mobilefinetuner_amd import layer_norm as L
+    x = torch.zeros(N, D, dtype=torch.bfloat16, device=dev)
+    last, w, b, dy = (t.to(dev) for t in make(5, D, "bf16", 15))
+    x[-5:] = last
+    y, mean, rstd = L.layer_norm(x, w, b)
+    ref = L.layer_norm(last, w, b)
+    assert all(torch.equal(p[-5:], q) for p, q in zip((y, mean, rstd), ref))
+    assert torch.equal(y[0], b.bfloat16()) and torch.equal(y[N - 6], y[0]) and (rstd[:-5] == rstd[0]).all()
+    if D > 16384:  # beyond the backward's registers
+        y.zero_()
+        y[-5:] = dy
+        dx = L.layer_norm_backward(x, w, mean, rstd, y, want_params=False)[0]
+        assert torch.equal(dx[-5:], L.layer_norm_backward(last, w, *ref[1:], dy, want_params=False)[0])
+        del dx
+    del x, y
+
+
+@pytest.mark.gpu
 def test_values_that_are_not_numbers_stay_in_their_row(dev):
     from mobilefinetuner_amd import layer_norm as L
     x, w, b, dy = (t.to(dev) for t in make(8, 257, "f32", 7))

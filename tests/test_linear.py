@@ -306,6 +306,34 @@ def test_values_that_are_not_numbers_stay_in_their_row(dev, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("N", [1, 40])
+def test_relu_of_infinities(dev, N, dtype):
+    from mobilefinetuner_amd import linear as L
+    x, W = torch.zeros(N, 8, dtype=DT[dtype], device=dev), torch.ones(8, 3, dtype=DT[dtype], device=dev)
+    y, z = L.linear(x, W, torch.tensor([-math.inf, math.inf, math.nan], device=dev), "relu", want_preact=True)
+    assert (y[:, 0] == 0).all() and (y[:, 1] == math.inf).all() and torch.isnan(y[:, 2]).all()
+    assert (z[:, 0] == -math.inf).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_most_rows(dev, dtype):
+    """2^29 rows, as many tiles as a launch takes: sums of two small whole numbers, exact in both types."""
+    from mobilefinetuner_amd import linear as L
+    N = 1 << 29
+    x = torch.zeros(N, 2, dtype=DT[dtype], device=dev)
+    x[-70:], x[:70] = 2, 1
+    W, b = torch.tensor([[1.0], [3.0]], device=dev).to(DT[dtype]), torch.ones(1, device=dev)
+    y = L.linear(x, W, b)[0]
+    assert (y[-70:] == 9).all() and (y[:70] == 5).all() and (y[70:-70] == 1).all()
+    dx, dW, db = L.linear_backward(x, W, None, y)
+    assert torch.equal(dx[-1], (9 * W[:, 0])) and torch.equal(dx[0], 5 * W[:, 0]) and torch.equal(dx[100], W[:, 0])
+    ref = 70 * (2 * 9 + 5)
+    assert (dW.float() - ref).abs().max() <= torch.finfo(DT[dtype]).eps / 2 * ref
+
+
+@pytest.mark.gpu
 def test_far_pre_activations(dev):
     """Activations and derivatives far from zero: no NaN, their limits."""
     from mobilefinetuner_amd import linear as L
@@ -443,6 +471,7 @@ def capi():
     (dict(N=-1), "N >= 0"), (dict(in_dim=0), "positive"), (dict(out_dim=-4), "positive"), (dict(dtype=1), "dtype"),
     (dict(activation=4), "activation"), (dict(activation=-1), "activation"), (dict(in_dim=1 << 25), "2\\^24"),
     (dict(N=1 << 31), "2\\^31"), (dict(N=1 << 24, in_dim=1 << 16), "too large"),
+    (dict(N=(1 << 29) + 1), "too large"),
 ])
 def test_descriptors_refused(capi, change, message):
     d = capi.linear_desc(**{**dict(N=4, in_dim=64, out_dim=32), **change})

@@ -303,6 +303,21 @@ def test_captured_graph_and_streams(dev, N, V):
         assert all(torch.equal(p, q) for p, q in zip(r, ref))
 
 
+@pytest.mark.gpu
+def test_the_most_rows(dev):
+    """2^24 - 1 rows: the last ones as in a call of their own."""
+    from mobilefinetuner_amd import logprobs as L
+    N = (1 << 24) - 1
+    z = torch.zeros(N, 3, dtype=torch.bfloat16, device=dev)
+    z[-5:] = torch.randn(5, 3, generator=torch.Generator().manual_seed(5)).to(dev)
+    t = torch.ones(N, dtype=torch.int32, device=dev)
+    got, ref = L.token_logprobs(z, t, 2), L.token_logprobs(z[-5:], t[-5:], 2)
+    assert all(torch.equal(p[-5:], q) for p, q in zip(got, ref))
+    one = torch.ones(N, device=dev)
+    g = L.token_logprobs_backward(z, t, got[2], got[1], one)
+    assert torch.equal(g[-5:], L.token_logprobs_backward(z[-5:], t[-5:], ref[2], ref[1], one[-5:]))
+
+
 # ------------------------------------------------------------------ refusals
 @pytest.fixture(scope="module")
 def capi():
@@ -312,7 +327,7 @@ def capi():
 
 
 @pytest.mark.parametrize("change,message", [
-    (dict(N=-1), "N >= 0"), (dict(V=0), "V > 0"), (dict(N=(1 << 24) + 1), "2\\^24"), (dict(V=(1 << 30) + 1), "2\\^30"),
+    (dict(N=-1), "N >= 0"), (dict(V=0), "V > 0"), (dict(N=(1 << 24) + 1), "2\\^24"), (dict(N=1 << 24), "2\\^24"), (dict(V=(1 << 30) + 1), "2\\^30"),
     (dict(dtype=1), "dtype"), (dict(top=-1), "top"), (dict(top=65), "top"), (dict(V=10, top=11), "top"),
     (dict(ld=99), "stride"), (dict(grad_ld=-100), "stride"),
 ])
