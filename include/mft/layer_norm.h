@@ -20,7 +20,7 @@
  * caller-owned device memory, stream ordering, no allocation), but rows may
  * start at any element: the base addresses need no more than the alignment of
  * their type, and row strides may be odd.  N may be 0 (the parameters'
- * gradients are then zero).
+ * gradients are then zero); it is below 2^31, and D at most 2^30.
  */
 #ifndef MFT_LAYER_NORM_H
 #define MFT_LAYER_NORM_H

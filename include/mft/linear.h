@@ -24,6 +24,8 @@
  * Conventions are those of mft/attention.h (status codes, mft_last_error,
  * caller-owned device memory, stream ordering, no allocation).  All operands
  * are contiguous.  N may be 0 (the gradients of W and bias are then zero).
+ * Refused: N of 2^31 or more, in and out above 2^24, and products of more than
+ * 2^23 tiles of 64 x 64.
  */
 #ifndef MFT_LINEAR_H
 #define MFT_LINEAR_H

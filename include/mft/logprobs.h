@@ -28,7 +28,7 @@
  *
  * Conventions are those of mft/attention.h (status codes, mft_last_error,
  * caller-owned device memory, stream ordering, no allocation), but rows may
- * start at any element.  N may be 0.
+ * start at any element.  N may be 0; it is below 2^24, and V at most 2^30.
  */
 #ifndef MFT_LOGPROBS_H
 #define MFT_LOGPROBS_H

@@ -600,7 +600,7 @@ struct Plan {
 // tile and cut into 1 to 8 slices: the choice by these is the fastest or within 6
 // percent of it but for three, the worst at 1.13 times it.
 //   256 x 128, two workgroups to a CU: heavy epilogues over short K.  8192 x 1024
-//     -> 4096 with GELU 94 us, 256 x 256 104, 128 x 128 112.
+//     -> 4096 with GELU 89 us, 256 x 256 104, 128 x 128 112.
 //   256 x 256, one wave to a SIMD with its accumulators in all of its registers:
 //     least LDS and L2 traffic per product.  8192^3 815 us (1350 TFLOP/s), 128 x
 //     128 980.
