@@ -13,8 +13,9 @@
  *   dz_j = grad_logprob[n] (1[j = tokens[n]] - p_j) - grad_entropy[n] p_j (log p_j + entropy[n])
  *
  * The logits and their gradient have element type `dtype`; all else is fp32,
- * as are the sums.  A probability of zero (a logit of -inf) adds nothing to the
- * entropy or its gradient.  A row that holds a NaN or +inf, or nothing but -inf,
+ * as are the sums.  A probability of zero (a logit of -inf, or one so far below
+ * the row's largest that exp is 0, as a mask of the type's lowest value is) adds
+ * nothing to the entropy or its gradient.  A row that holds a NaN or +inf, or nothing but -inf,
  * has NaN log probabilities and entropy; NaN logits are never alternatives
  * (top_ids is -1 where a row has fewer numbers than `top`).
  *

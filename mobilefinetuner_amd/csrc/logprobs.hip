@@ -37,14 +37,16 @@ constexpr int kUnroll = 8;
 constexpr int kBwdVecs = 4;  // of a thread of the backward's workgroups
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
 constexpr float kLowest = -1e30f;  // in place of -inf in a product with a probability of 0
+constexpr float kGone = -1e6f;     // exp is 0 from here down, and its product with a sum (at most 2^30) finite
 
 struct Sums {
     float m = -INFINITY, s = 0.f, t = 0.f;
-    // The sums about a larger maximum.
+    // The sums about a larger maximum.  Logits excluded by a type's lowest value are up to
+    // 3.4e38 below it: their s (m - to) would overflow, and f = 0 make NaN of that.
     __device__ __forceinline__ void move_to(float to) {
         if (m != -INFINITY) {  // else s and t are 0, or the NaN of a value
             const float f = __expf(m - to);
-            t = f * fmaf(s, m - to, t);
+            t = f * fmaf(s, fmaxf(m - to, kGone), t);
             s *= f;
         }
         m = to;

@@ -152,6 +152,43 @@ def test_excluded_logits(dev, V, dtype):
     assert (lp == -math.inf).all()
 
 
+# one workgroup to a row below 8192, or with more rows than half the workgroups; parts of one else
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,V", [(6, 300), (6, 5000), (6, 70001), (1030, 9000), (6, 262144)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lowest", ["finfo.min", -1e38, -1e35, -1e30])
+def test_logits_excluded_by_a_finite_value(dev, lowest, dtype, N, V):
+    """Their probability is 0, and they add nothing to the entropy or the gradient, whoever meets them first
+    or alone: a thread, a wave, a part."""
+    from mobilefinetuner_amd import logprobs as L
+    print(f"[case] {N} x {V} {dtype} {lowest}", flush=True)
+    low = torch.finfo(DT[dtype]).min if lowest == "finfo.min" else lowest
+    z, t, gl, ge = make(N, V, dtype, V)
+    live = torch.zeros(6, V, dtype=torch.bool)
+    live[0, V // 2] = True                            # one value, of one thread
+    live[1, :10] = True                               # the first ones
+    live[2, -(V // 3):] = True                        # behind what is masked
+    live[3, ::7] = True                               # in every vector
+    live[4] = torch.arange(V) // 8 % 256 >= 128       # of every other wave or two; none of 300
+    live[5] = torch.arange(V) // 1024 % 2 == 1        # rounds of vectors
+    live[5, -1] = True
+    live = live.repeat(N // 6 + 1, 1)[:N]
+    z[~live] = low
+    t = torch.where(torch.arange(N) % 2 == 0, live.int().argmax(1), t.long()).int()
+    stats, ent = check_forward(z, t, min(20, V), dev)
+    assert torch.isfinite(ent).all() and (ent[0::6] == 0).all()
+    g = L.token_logprobs_backward(z.to(dev), t.to(dev), stats, ent, gl.to(dev), ge.to(dev)).cpu()
+    within(g, *ref_backward(z, t, stats.cpu(), ent.cpu(), gl, ge))
+    some = live.any(1)  # row 4 of 300 has nothing else: the uniform distribution
+    masked = ~live & some[:, None]
+    masked.scatter_(1, t.long()[:, None], False)
+    assert (g[masked] == 0).all()
+    # the sums are those of a row with -inf in their place
+    z[~live] = -math.inf
+    _, e2, s2, _, _ = L.token_logprobs(z.to(dev), t.to(dev))
+    assert torch.equal(s2[some], stats[some]) and torch.equal(e2[some], ent[some])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("V", [300, 9000, 60000])
 def test_rows_without_a_distribution(dev, V):
