@@ -348,7 +348,7 @@ template <typename T> __global__ __launch_bounds__(kLpThreads) void lp_bwd(Logpr
     const int64_t yl = on ? y - lo : -1;
     auto grad = [&](float x, int i) {
         const float q = (x - s.x) - s.y, p = __expf(q);
-        const float v = -p * fmaf(ge, fmaxf(q, kLowest) + entropy, gl);
+        const float v = p == 0.f ? 0.f : -p * fmaf(ge, q + entropy, gl);  // no 0 * inf, and a NaN stays
         return i == yl ? v + gl : v;
     };
     for (int j = threadIdx.x; j < nvec; j += NT) {

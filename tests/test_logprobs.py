@@ -190,6 +190,28 @@ def test_logits_excluded_by_a_finite_value(dev, lowest, dtype, N, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [300, 70001])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("large", [1e9, 1e20, 1e30])
+def test_large_entropy_gradients_of_excluded_logits(dev, large, dtype, V):
+    """A probability of 0 adds nothing however large the entropy's gradient is; one that is lost below
+    2^-126 is a logit at most 104 under the largest."""
+    from mobilefinetuner_amd import logprobs as L
+    print(f"[case] {large} {dtype} {V}", flush=True)
+    z, t, gl, ge = make(4, V, dtype, V)
+    ge = large * torch.tensor([1.0, -1.0, 0.5, -0.3])
+    z[0, ::3], z[1, ::3], z[2, 5:] = -math.inf, torch.finfo(DT[dtype]).min, -200.0
+    t = torch.tensor([1, 0, 7, V - 1], dtype=torch.int32)  # row 1's and 2's are excluded ones
+    _, ent, stats, _, _ = L.token_logprobs(z.to(dev), t.to(dev))
+    g = L.token_logprobs_backward(z.to(dev), t.to(dev), stats, ent, gl.to(dev), ge.to(dev)).cpu()
+    ref, tol = ref_backward(z, t, stats.cpu(), ent.cpu(), gl, ge)
+    lost = 2.0 ** -126 * (gl.abs() + ge.abs() * (104 + ent.cpu()))
+    within(g, ref, tol + lost.double()[:, None])
+    assert g[1, 0] == gl[1].to(z.dtype) and g[2, 7] == gl[2].to(z.dtype)
+    assert (g[0, ::3] == 0).all() and (g[1, 3::3] == 0).all() and (g[2, 8:] == 0).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [300, 9000, 60000])
 def test_rows_without_a_distribution(dev, V):
     """Nothing but -inf, a NaN, +inf: NaN in that row alone; alternatives are its numbers."""
