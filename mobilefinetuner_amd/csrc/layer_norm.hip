@@ -324,12 +324,12 @@ template <typename T> __global__ __launch_bounds__(256) void ln_bwd_columns(Laye
     }
 }
 
-// dw and db: the groups' partials in order.  32 columns (a line) to a workgroup;
-// its 32 rows of threads take the groups in turn.
-__global__ __launch_bounds__(1024) void ln_params(LayerNormArgs a) {
+// dw and db from column `first` of the two on: the groups' partials in order.  32
+// columns (a line) to a workgroup; its 32 rows of threads take the groups in turn.
+__global__ __launch_bounds__(1024) void ln_params(LayerNormArgs a, int64_t first) {
     __shared__ float s[32][33];
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * 32 + x, C = 2 * a.D;
+    const int64_t c = first + (int64_t)blockIdx.x * 32 + x, C = 2 * a.D;
     float v = 0.f;
     if (c < C)
 #pragma unroll 8
@@ -458,7 +458,10 @@ template <typename T> hipError_t bwd(const LayerNormArgs& a, hipStream_t st) {
 #undef MFT_LN_BWD
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !params) return e;
-    hipLaunchKernelGGL(ln_params, dim3((unsigned)((2 * a.D + 31) / 32)), dim3(1024), 0, st, a);
+    // 32 threads to a column of the two: 2^26 columns at a time (from D = 2^26 on a launch's 2^32 threads were too few)
+    constexpr int64_t kMost = int64_t(1) << 26;
+    for (int64_t c = 0; c < 2 * a.D; c += kMost)
+        hipLaunchKernelGGL(ln_params, dim3((unsigned)((std::min(kMost, 2 * a.D - c) + 31) / 32)), dim3(1024), 0, st, a, c);
     return hipGetLastError();
 }
 

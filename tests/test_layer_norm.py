@@ -206,6 +206,28 @@ def test_more_rows_than_a_launch_takes(dev, N, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [(1 << 25) + 33, 1 << 26, (1 << 26) + 4099])
+def test_wider_rows_than_a_launch_takes(dev, D):
+    """The parameters' gradients on either side of a launch's columns.  Multiples of 1/2 whose sums stay below
+    2^23 (a thread's share of a row is some 2^16 products of at most 50, of mean zero): all sums are exact, and
+    dx has the roundings of its last few operations."""
+    from mobilefinetuner_amd import layer_norm as L
+    print(f"[case] D {D}", flush=True)
+    j = torch.arange(D, device=dev)
+    x = torch.stack([j % 13 - 6, j % 7 - 3]).bfloat16()
+    dy = torch.stack([j % 5 - 2, j % 11 - 5]).bfloat16()
+    mean, rstd = torch.tensor([1.0, -2.0], device=dev), torch.tensor([0.5, 2.0], device=dev)
+    dx, dw, db = L.layer_norm_backward(x, None, mean, rstd, dy)
+    h = (x.float() - mean[:, None]) * rstd[:, None]
+    assert torch.equal(db, dy.float().sum(0)) and torch.equal(dw, (dy.float() * h).sum(0))
+    c1, c2 = (dy.double().mean(1, keepdim=True), (dy.double() * h.double()).mean(1, keepdim=True))
+    ref = rstd.double()[:, None] * (dy.double() - c1 - h.double() * c2)
+    tol = 8 * U * rstd.double()[:, None] * (dy.abs() + c1.abs() + (h * c2).abs()) + half_step(x.dtype) * ref.abs()
+    assert bool(((dx.double() - ref).abs() <= tol).all())
+    del x, dy, dx, h, ref, tol
+
+
+@pytest.mark.gpu
 def test_values_that_are_not_numbers_stay_in_their_row(dev):
     from mobilefinetuner_amd import layer_norm as L
     x, w, b, dy = (t.to(dev) for t in make(8, 257, "f32", 7))
