@@ -9,6 +9,7 @@ memory out again only in its order.
 from __future__ import annotations
 
 import contextlib
+import functools
 
 import torch
 
@@ -76,3 +77,42 @@ def rows(t, last):
 
 def workspace(nbytes, like):
     return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+class _NoSecondDerivative(torch.autograd.Function):
+    """The first `n` tensors, gradients that kernels have computed, as functions of the others, whose derivative raises."""
+
+    @staticmethod
+    def forward(ctx, name, n, *tensors):
+        ctx.name = name
+        ctx.mark_dirty(*tensors[:n])
+        return tensors[:n]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name}: its gradients have no derivative (no second order)")
+
+
+def first_order(backward):
+    """Decorates the backward of a node whose gradients the kernels compute.  With create_graph they
+    depend on the incoming gradients and on what the forward saved (and on ctx.also, where it
+    is set), and a derivative through them raises rather than leaving these terms out.  A gradient handed
+    on as it came in keeps its graph."""
+    name = backward.__qualname__.split(".")[0]
+
+    @functools.wraps(backward)
+    def checked(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        of = [t for t in (*grads, *ctx.saved_tensors, getattr(ctx, "also", None)) if t is not None and t.requires_grad]
+        own = [i for i, t in enumerate(out) if t is not None and not any(t is g for g in grads)]
+        if not of or not own:
+            return out
+        out = list(out)
+        for i, t in zip(own, _NoSecondDerivative.apply(name, len(own), *(out[i] for i in own), *of)):
+            out[i] = t
+        return tuple(out)
+
+    return checked

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import capi
-from .device import DTYPES, guard, like, operand, optional, ptr, rows, stream, workspace
+from .device import DTYPES, first_order, guard, like, operand, optional, ptr, rows, stream, workspace
 
 
 def _param(p, name, x):
@@ -66,6 +66,7 @@ class LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import capi
-from .device import DTYPES, guard, like, operand, ptr, stream, workspace
+from .device import DTYPES, first_order, guard, like, operand, ptr, stream, workspace
 
 ACTIVATIONS = {"none": capi.MFT_ACT_NONE, "relu": capi.MFT_ACT_RELU, "gelu_tanh": capi.MFT_ACT_GELU_TANH,
                "silu": capi.MFT_ACT_SILU}
@@ -87,10 +87,12 @@ class Linear(torch.autograd.Function):
         y, z = linear(x, W, bias, activation, residual, w_transposed,
                       activation != "none" and (need[0] or need[1] or need[2]))
         ctx.save_for_backward(x, W, z)
+        ctx.also = bias if z is not None else None  # z is a function of it, too
         ctx.cfg = (activation, w_transposed)
         return y
 
     @staticmethod
+    @first_order
     def backward(ctx, dy):
         x, W, z = ctx.saved_tensors
         need = ctx.needs_input_grad

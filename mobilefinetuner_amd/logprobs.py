@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import capi
-from .device import DTYPES, guard, like, operand, optional, ptr, rows, stream, workspace
+from .device import DTYPES, first_order, guard, like, operand, optional, ptr, rows, stream, workspace
 
 
 def _operands(logits, tokens):
@@ -77,6 +77,7 @@ class TokenLogprobs(torch.autograd.Function):
         return logprob, entropy
 
     @staticmethod
+    @first_order
     def backward(ctx, grad_logprob, grad_entropy):
         if grad_logprob is None and grad_entropy is None:
             return None, None, None, None
