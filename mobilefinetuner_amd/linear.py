@@ -81,11 +81,16 @@ def linear_backward(x, W, z, dy, activation="none", w_transposed=False, want_x=T
 class Linear(torch.autograd.Function):
     """y = Linear.apply(x, W, bias, residual, activation, w_transposed)."""
 
+    @classmethod
+    def apply(cls, x, W, bias=None, residual=None, activation="none", w_transposed=False):
+        # Whether a backward can follow is seen here alone: needs_input_grad is the leaves', also under no_grad.
+        return super().apply(x, W, bias, residual, activation, w_transposed, torch.is_grad_enabled())
+
     @staticmethod
-    def forward(ctx, x, W, bias=None, residual=None, activation="none", w_transposed=False):
+    def forward(ctx, x, W, bias, residual, activation, w_transposed, grad_mode):
         need = ctx.needs_input_grad
         y, z = linear(x, W, bias, activation, residual, w_transposed,
-                      activation != "none" and (need[0] or need[1] or need[2]))
+                      grad_mode and activation != "none" and (need[0] or need[1] or need[2]))
         ctx.save_for_backward(x, W, z)
         ctx.also = bias if z is not None else None  # z is a function of it, too
         ctx.cfg = (activation, w_transposed)
@@ -100,4 +105,4 @@ class Linear(torch.autograd.Function):
         if need[0] or need[1] or need[2]:
             dx, dW, db = linear_backward(x, W, z, dy, *ctx.cfg, want_x=need[0], want_weight=need[1],
                                          want_bias=need[2])
-        return dx, dW, db, dy if need[3] else None, None, None
+        return dx, dW, db, dy if need[3] else None, None, None, None

@@ -144,3 +144,23 @@ def test_nothing_to_differentiate_stays_without_a_graph(place):
     y = Linear.apply(x, W, None, r, "none", False)
     y.sum().backward()
     assert not any(t.grad.requires_grad for t in (x, W, r))
+
+
+def test_the_pre_activation_is_kept_for_a_backward_only(place, monkeypatch):
+    """Not under no_grad or inference_mode, nor where only the residual is trained."""
+    from mobilefinetuner_amd import linear as L
+    asked, real = [], L.linear
+    monkeypatch.setattr(L, "linear", lambda *a, **k: (asked.append(a[6] if len(a) > 6 else k.get("want_preact", False)),
+                                                      real(*a, **k))[1])
+    x, W, b, r = leaves(place, (5, 24), (24, 16), (16,), (5, 16))
+    y = L.Linear.apply(x, W, b, r, "silu")
+    with torch.no_grad():
+        quiet = L.Linear.apply(x, W, b, r, "silu", False)
+    with torch.inference_mode():
+        L.Linear.apply(x, W, b, r, "silu", False)
+    L.Linear.apply(x.detach(), W.detach(), b.detach(), r, "silu")
+    L.Linear.apply(x, W, b)
+    assert asked == [True, False, False, False, False]
+    assert torch.equal(quiet, y) and not quiet.requires_grad
+    y.sum().backward()
+    assert all(t.grad is not None for t in (x, W, b, r))
