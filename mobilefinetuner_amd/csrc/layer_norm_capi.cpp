@@ -44,6 +44,8 @@ mft_status mft_layer_norm_fwd(const mft_layer_norm_desc* desc, const void* x, co
     const mft_status r = check(desc, "mft_layer_norm_fwd", &a);
     if (r != MFT_OK) return r;
     if (desc->N > 0 && (!x || !y)) return fail(MFT_ERR_INVALID_ARG, "mft_layer_norm_fwd: x and y must be non-NULL");
+    if (desc->N > 1 && y == x && a.sy != a.sx)
+        return fail(MFT_ERR_INVALID_ARG, "mft_layer_norm_fwd: y in place needs x's row stride");
     a.x = x;
     a.w = weight;
     a.b = bias;
@@ -70,6 +72,8 @@ mft_status mft_layer_norm_bwd(const mft_layer_norm_desc* desc, const void* x, co
     if (desc->N > 0 && (!x || !mean || !rstd || !dy || !workspace))
         return fail(MFT_ERR_INVALID_ARG, "mft_layer_norm_bwd: x, mean, rstd, dy and workspace must be non-NULL");
     if (desc->N > 0 && dx == x) return fail(MFT_ERR_INVALID_ARG, "mft_layer_norm_bwd: dx may not be x");
+    if (desc->N > 1 && dx == dy && a.sdx != a.sdy)
+        return fail(MFT_ERR_INVALID_ARG, "mft_layer_norm_bwd: dx in place needs dy's row stride");
     a.x = x;
     a.w = weight;
     a.mean_in = mean;

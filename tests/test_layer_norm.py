@@ -355,6 +355,14 @@ def test_null_and_aliased_operands_refused(capi):
                                          None) == capi.MFT_OK
 
 
+def test_in_place_with_other_strides_refused(capi):
+    """Rows would be overwritten before they are read."""
+    with pytest.raises(capi.MftError, match="in place"):
+        capi.layer_norm_fwd(capi.layer_norm_desc(4, 64, x_stride=80), 16, None, None, 16, None, None, None)
+    with pytest.raises(capi.MftError, match="in place"):
+        capi.layer_norm_bwd(capi.layer_norm_desc(4, 64, dx_stride=80), 16, None, 32, 48, 64, 64, None, None, 96, None)
+
+
 def test_no_cpu_path():
     from mobilefinetuner_amd import layer_norm as L
     with pytest.raises(ValueError, match="no CPU path"):
