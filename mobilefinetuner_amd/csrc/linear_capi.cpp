@@ -136,7 +136,7 @@ mft_status mft_linear_fwd(const mft_linear_desc* desc, const void* x, const void
     if (!x || !W || !y) return fail(MFT_ERR_INVALID_ARG, "mft_linear_fwd: x, W and y must be non-NULL");
     if (z && desc->activation == MFT_ACT_NONE)
         return fail(MFT_ERR_INVALID_ARG, "mft_linear_fwd: z is kept with an activation only");
-    if (y == x || y == W || (z && (z == y || z == x || z == residual)))
+    if (y == x || y == W || (z && (z == y || z == x || z == W || z == residual)))
         return fail(MFT_ERR_INVALID_ARG, "mft_linear_fwd: y may not be x or W, nor z another operand");
     char* ws = static_cast<char*>(workspace);
     const bool bf = desc->dtype == MFT_BF16;
@@ -175,6 +175,7 @@ mft_status mft_linear_bwd(const mft_linear_desc* desc, const void* x, const void
                                          "activation) must be non-NULL");
     if ((dx && (dx == dy || dx == x || dx == W || dx == z)) || (dW && (dW == W || dW == x || dW == dy || dW == z)))
         return fail(MFT_ERR_INVALID_ARG, "mft_linear_bwd: dx and dW may not be operands");
+    if (dx && dx == dW) return fail(MFT_ERR_INVALID_ARG, "mft_linear_bwd: dx and dW may not be one tensor");
     const BwdLayout l = bwd_layout(desc);
     char* ws = static_cast<char*>(workspace);
     const void* dz = act ? ws + l.dz : dy;

@@ -512,6 +512,15 @@ def test_null_and_aliased_operands_refused(capi, dtype):
     assert capi.lib().mft_linear_bwd(C.byref(act), 16, 32, 48, 64, None, None, None, 128, None) == capi.MFT_OK
 
 
+@pytest.mark.parametrize("dtype", [0, 2])
+def test_outputs_over_weights_or_each_other_refused(capi, dtype):
+    d = capi.linear_desc(4, 64, 32, dtype, False, capi.MFT_ACT_SILU)
+    with pytest.raises(capi.MftError, match="may not be"):
+        capi.linear_fwd(d, 16, 32, None, None, 48, 32, 64, None)
+    with pytest.raises(capi.MftError, match="may not be one"):
+        capi.linear_bwd(d, 16, 32, 48, 64, 80, 80, None, 128, None)
+
+
 def test_no_cpu_path():
     from mobilefinetuner_amd import linear as L
     with pytest.raises(ValueError, match="no CPU path"):
