@@ -412,6 +412,8 @@ def linear_bwd(d, x, W, z, dy, dx, dW, dbias, workspace, stream) -> None:
 
 
 def logprobs_desc(N, V, ld=0, grad_ld=0, dtype=MFT_F32, ignore_index=-100, top=0):
+    if not -2 ** 31 <= ignore_index < 2 ** 31:  # ctypes would take its low 32 bits
+        raise ValueError(f"ignore_index must fit in int32, as the tokens do, got {ignore_index}")
     return LogprobsDesc(N, V, ld, grad_ld, dtype, ignore_index, top)
 
 

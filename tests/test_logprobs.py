@@ -422,6 +422,15 @@ def test_null_operands_refused(capi):
     assert capi.lib().mft_logprobs_fwd(C.byref(empty), *[None] * 10) == capi.MFT_OK
 
 
+@pytest.mark.parametrize("wrong", [2 ** 32 - 100, 2 ** 31, -2 ** 31 - 1])
+def test_an_ignore_index_beyond_the_tokens_type_refused(capi, wrong):
+    """Its low 32 bits are another token's."""
+    with pytest.raises(ValueError, match="int32"):
+        capi.logprobs_desc(4, 100, ignore_index=wrong)
+    for most in (2 ** 31 - 1, -2 ** 31):
+        assert capi.logprobs_desc(4, 100, ignore_index=most).ignore_index == most
+
+
 def test_no_cpu_path():
     from mobilefinetuner_amd import logprobs as L
     with pytest.raises(ValueError, match="no CPU path"):
