@@ -69,15 +69,6 @@ __device__ __forceinline__ float wave_sum_f(float x) {
     x = row16_sum(x);
     return half_sum(x);
 }
-__device__ __forceinline__ float wave_max_f(float x) {
-    x = fmaxf(x, dpp<0xB1>(x));
-    x = fmaxf(x, dpp<0x4E>(x));
-    x = fmaxf(x, dpp<0x141>(x));
-    x = fmaxf(x, dpp<0x140>(x));
-    x = row16_max(x);
-    return half_max(x);
-}
-
 
 // x of lane (lane ^ O), in registers: quads, halves and rows of 16 by DPP, the
 // rest by lane swaps.  All lanes must be active.
