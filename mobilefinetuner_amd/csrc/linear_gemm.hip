@@ -684,11 +684,14 @@ template <int ACT> void launch_act_fwd(const Plan& p, bool dma, hipStream_t st) 
 }
 
 // Operands whose rows are off 16 bytes are first copied to rows of whole ones,
-// where the product (of M N K pairs of numbers) is worth up to two more launches:
-// 5000 x 600 -> 1500 with W [in, out] 38 -> 25 us, its dW 56 -> 29; 300 x 600 ->
-// 1501 17 -> 11.  With k contiguous in the operands that are off, the registers'
-// way is less slow: 300 x 1501 by [600, 1501] 11.5 us, copied 17.
-constexpr double kPackWorth = 1e8, kPackWorthKc = 1.5e9;
+// where the product (of M N K pairs of numbers) is worth up to two more launches.
+// 47 sizes, each product copied and through the registers, on operands out of
+// cache: from 4e8 on copies take 0.3 to 1.1 times as long in most (4e8 to 1e9,
+// at most 1.5), 2000 x 1153 -> 2001 41 -> 26 us, its dW 67 -> 28; under 3e8 1.1 to
+// 1.9 times in most, 120 x 900 -> 1100's dW 7 -> 11.  With k contiguous in the
+// operands that are off the registers' way is less slow: 1.0 to 1.3 times from
+// 1e9 to 2e9, 0.7 to 1.1 above.
+constexpr double kPackWorth = 4e8, kPackWorthKc = 2e9;
 size_t up(size_t x) { return (x + 255) & ~size_t(255); }
 int64_t whole_ld(int64_t cols) { return (cols + 7) / 8 * 8; }
 struct Packs {
