@@ -155,7 +155,8 @@ template <int BN, int BM> __device__ __forceinline__ void place(const Args& a, i
     *slice = __builtin_amdgcn_readfirstlane((int)a.per_slice_tiles.div(i));
     i -= *slice * a.tiles_m * a.tiles_n;
     // Four rows of tiles at a time (of 256, eight), column by column: 8192 x 1024 -> 4096 with GELU, 256 x
-    // 128, 94 us with eight, 89 with four; 256 x 256 is up to 1 percent the other way.
+    // 128, 98 us with eight, 92 with four (its plain y 76 and 78, dW 71 and 69); of 13 other products none
+    // is off by over 1 percent either way.
     constexpr int kBand = BM > 128 ? 8 : 4;
     const int band = i / (kBand * a.tiles_n), in = i - band * kBand * a.tiles_n;
     const int high = min(kBand, a.tiles_m - band * kBand), col = in / high;
@@ -595,18 +596,18 @@ struct Plan {
 
 // The tiles, and what each sustains over the whole GPU (TFLOP/s) with one
 // workgroup to a CU and with more, and the k that its prologue and epilogue are
-// worth (with an activation: `act` more).  Fitted to 51 products of 16 to 8192
-// rows and 640 to 6912 columns, each timed on operands out of cache in every
-// tile and cut into 1 to 8 slices: the choice by these is the fastest or within 6
-// percent of it but for three, the worst at 1.13 times it.
+// worth (with an activation: `act` more).  Fitted to products of 16 to 8192 rows
+// and 600 to 6912 columns, each timed on operands out of cache in every tile and
+// cut into 1 to 16 slices: of 54 the choice by these is the fastest or within 6
+// percent of it in 49, within 8 in 53, and 1.16 times it in one.
 //   256 x 128, two workgroups to a CU: heavy epilogues over short K.  8192 x 1024
-//     -> 4096 with GELU 89 us, 256 x 256 104, 128 x 128 112.
+//     -> 4096 with GELU 88 us, 256 x 256 97, 128 x 128 104.
 //   256 x 256, one wave to a SIMD with its accumulators in all of its registers:
-//     least LDS and L2 traffic per product.  8192^3 815 us (1350 TFLOP/s), 128 x
-//     128 980.
-//   deep: 8192 x 1024 -> 4096's dW (256 tiles of 128 x 128 over K 8192) 79 us, 104
-//     with one workgroup of 4 waves to a CU; its dx in 256 x 128 63 us for 71 in
-//     128 x 128; 4096 x 6912 -> 1152 in 192 x 128 79 us for 96.
+//     least LDS and L2 traffic per product.  8192^3 844 us (1300 TFLOP/s), 256 x
+//     128 923, 128 x 128 1025; W [out, in] 808, 128 x 128 946.
+//   deep: 8192 x 1024 -> 4096's dW (256 tiles of 128 x 128 over K 8192) 78 us, 113
+//     with one workgroup of 4 waves to a CU; its dx in 256 x 128 63 us for 74 in
+//     128 x 128; 4096 x 6912 -> 1152 in 192 x 128 79 us (with a residual 85) for 98.
 // With k contiguous in both operands the slabs of 256 x 128 do not leave a CU
 // room for two; a slab of 192 rows has no whole direct loads without.
 struct Shape {

@@ -9,9 +9,9 @@
 // Q with k contiguous: a wave takes four rows of Q, or one where that leaves
 // fewer than four waves to a CU, and its lanes share k.  Q with its rows
 // contiguous: a workgroup takes 64 consecutive n or fewer (so that about 128
-// workgroups run) and its lanes' groups share k.  bf16, one row, calls back to
-// back: 1024 -> 4096 4.1 us (W [out, in]) and 4.9 ([in, out]), 4096 -> 1024 4.8
-// and 6.4; on 64 x 64 tiles of the matrix units 6.0, 7.0, 9.0 and 9.3.
+// workgroups run) and its lanes' groups share k.  bf16, one row, W out of cache:
+// 1024 -> 4096 5.7 us (W [out, in]) and 6.2 ([in, out]), 4096 -> 1024 6.9 and 10.6;
+// on 64 x 64 tiles of the matrix units 8.6, 8.9, 10.6 and 10.6.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -26,7 +26,9 @@ namespace mft {
 namespace {
 
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
-// Four rows of 4096 -> 1024 take 13 us here and 10 on the matrix units.
+// Against the tiles of the matrix units, on operands out of cache, eight layers of 768 to 8192: one row
+// 4.5 to 13.5 us for 8 to 13, two 4.5 to 15.6 for 8 to 13 (over K of 4096 and more up to a quarter
+// longer here, else shorter), three 11 to 21 for 9 to 13 with W [in, out].
 constexpr int kMaxRows = 2;
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 

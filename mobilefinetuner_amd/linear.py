@@ -5,7 +5,10 @@ forward and backward, over the C ABI of include/mft/linear.h.
 
 x [..., in], W [in, out] or, with w_transposed, [out, in], residual and y
 [..., out] are all fp32 or all bf16; bias [out] and its gradient are fp32.  act
-is "none", "relu", "gelu_tanh" or "silu".  There is no CPU path.
+is "none", "relu", "gelu_tanh" or "silu".  Operands that are not contiguous are
+copied on every call: pass a weight stored [out, in] with w_transposed, not its
+transposed view.  In bf16 the backward rounds dz = dy act'(z) to bf16 for both
+products, with an activation.  There is no CPU path.
 """
 from __future__ import annotations
 
