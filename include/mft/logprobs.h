@@ -15,9 +15,9 @@
  * The logits and their gradient have element type `dtype`; all else is fp32,
  * as are the sums.  A probability of zero (a logit of -inf, or one so far below
  * the row's largest that exp is 0, as a mask of the type's lowest value is) adds
- * nothing to the entropy or its gradient.  A row that holds a NaN or +inf, or nothing but -inf,
- * has NaN log probabilities and entropy; NaN logits are never alternatives
- * (top_ids is -1 where a row has fewer numbers than `top`).
+ * nothing to the entropy or its gradient.  A row that holds a NaN or +inf, or
+ * nothing but -inf, has NaN log probabilities and entropy; NaN logits are never
+ * alternatives (top_ids is -1 where a row has fewer numbers than `top`).
  *
  * Rows whose token is ignore_index are not read: logprob, entropy and stats are
  * 0, top_logprobs -inf, top_ids -1, and the gradient is 0.  A token outside

@@ -458,7 +458,7 @@ template <typename T> hipError_t bwd(const LayerNormArgs& a, hipStream_t st) {
 #undef MFT_LN_BWD
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !params) return e;
-    // 32 threads to a column of the two: 2^26 columns at a time (from D = 2^26 on a launch's 2^32 threads were too few)
+    // 32 threads to a column of the two, and fewer than 2^32 to a launch: 2^26 columns at a time
     constexpr int64_t kMost = int64_t(1) << 26;
     for (int64_t c = 0; c < 2 * a.D; c += kMost)
         hipLaunchKernelGGL(ln_params, dim3((unsigned)((std::min(kMost, 2 * a.D - c) + 31) / 32)), dim3(1024), 0, st, a, c);
