@@ -37,6 +37,10 @@ LAYER_EXPORTS = (
     "mft_linear_workspace_size", "mft_linear_fwd", "mft_linear_bwd",
     "mft_logprobs_workspace_size", "mft_logprobs_fwd", "mft_logprobs_bwd",
 )
+# The same of the gated half of a block and its training step: rms_norm.h, gated_linear.h and adamw.h.
+BLOCK_EXPORTS = (
+    "mft_rms_norm_fwd", "mft_rms_norm_e4m3_fwd", "mft_rms_norm_workspace_size", "mft_rms_norm_bwd",
+)
 LOGPROBS_MAX_TOP = 64
 MFT_ACT_NONE, MFT_ACT_RELU, MFT_ACT_GELU_TANH, MFT_ACT_SILU = 0, 1, 2, 3
 MFT_REDUCE_MEAN, MFT_REDUCE_SUM, MFT_REDUCE_NONE = 0, 1, 2
@@ -101,6 +105,12 @@ class LinearDesc(C.Structure):
 class LogprobsDesc(C.Structure):
     _fields_ = [("N", C.c_int64), ("V", C.c_int64), ("ld", C.c_int64), ("grad_ld", C.c_int64), ("dtype", C.c_int32),
                 ("ignore_index", C.c_int32), ("top", C.c_int32)]
+
+
+class RmsNormDesc(C.Structure):
+    _fields_ = [("N", C.c_int64), ("D", C.c_int64), ("dtype", C.c_int32), ("norm", C.c_int32), ("eps", C.c_float)] + \
+        [(n, C.c_int64) for n in ("x_stride", "residual_stride", "total_stride", "y_stride", "dy_stride",
+                                  "dtotal_stride", "dx_stride")]
 
 
 class MftError(RuntimeError):
@@ -187,6 +197,14 @@ def lib():
     L.mft_logprobs_fwd.argtypes = [C.POINTER(LogprobsDesc)] + [vp] * 10
     L.mft_logprobs_bwd.restype = C.c_int
     L.mft_logprobs_bwd.argtypes = [C.POINTER(LogprobsDesc)] + [vp] * 8
+    L.mft_rms_norm_fwd.restype = C.c_int
+    L.mft_rms_norm_fwd.argtypes = [C.POINTER(RmsNormDesc)] + [vp] * 7
+    L.mft_rms_norm_e4m3_fwd.restype = C.c_int
+    L.mft_rms_norm_e4m3_fwd.argtypes = [C.POINTER(RmsNormDesc)] + [vp] * 7
+    L.mft_rms_norm_workspace_size.restype = C.c_int
+    L.mft_rms_norm_workspace_size.argtypes = [C.POINTER(RmsNormDesc), C.POINTER(C.c_size_t)]
+    L.mft_rms_norm_bwd.restype = C.c_int
+    L.mft_rms_norm_bwd.argtypes = [C.POINTER(RmsNormDesc)] + [vp] * 9
     if L.mft_version() != 7:
         raise RuntimeError("libmft_attn.so version mismatch")
     _lib = L
@@ -431,3 +449,28 @@ def logprobs_fwd(d, logits, tokens, logprob, entropy, stats, top_logprobs, top_i
 def logprobs_bwd(d, logits, tokens, stats, entropy, grad_logprob, grad_entropy, grad_logits, stream) -> None:
     check(lib().mft_logprobs_bwd(C.byref(d), logits, tokens, stats, entropy, grad_logprob, grad_entropy, grad_logits,
                                  stream))
+
+
+def rms_norm_desc(N, D, dtype=MFT_F32, norm=MFT_NORM_GEMMA, eps=1e-6, x_stride=0, residual_stride=0, dy_stride=0,
+                  dtotal_stride=0, total_stride=0, y_stride=0, dx_stride=0):
+    """Row strides in elements (0 = D)."""
+    return RmsNormDesc(N, D, dtype, norm, eps, x_stride, residual_stride, total_stride, y_stride, dy_stride,
+                       dtotal_stride, dx_stride)
+
+
+def rms_norm_fwd(d, x, residual, weight, total, y, rstd, stream) -> None:
+    check(lib().mft_rms_norm_fwd(C.byref(d), x, residual, weight, total, y, rstd, stream))
+
+
+def rms_norm_e4m3_fwd(d, x, residual, weight, total, q, scale, stream) -> None:
+    check(lib().mft_rms_norm_e4m3_fwd(C.byref(d), x, residual, weight, total, q, scale, stream))
+
+
+def rms_norm_workspace_size(d) -> int:
+    n = C.c_size_t()
+    check(lib().mft_rms_norm_workspace_size(C.byref(d), C.byref(n)))
+    return n.value
+
+
+def rms_norm_bwd(d, x, weight, rstd, dy, dtotal, dx, dweight, workspace, stream) -> None:
+    check(lib().mft_rms_norm_bwd(C.byref(d), x, weight, rstd, dy, dtotal, dx, dweight, workspace, stream))
