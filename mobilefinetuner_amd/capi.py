@@ -40,8 +40,10 @@ LAYER_EXPORTS = (
 # The same of the gated half of a block and its training step: rms_norm.h, gated_linear.h and adamw.h.
 BLOCK_EXPORTS = (
     "mft_rms_norm_fwd", "mft_rms_norm_e4m3_fwd", "mft_rms_norm_workspace_size", "mft_rms_norm_bwd",
+    "mft_adamw_workspace_size", "mft_adamw_step",
 )
 LOGPROBS_MAX_TOP = 64
+ADAMW_GROUP = 256
 MFT_ACT_NONE, MFT_ACT_RELU, MFT_ACT_GELU_TANH, MFT_ACT_SILU = 0, 1, 2, 3
 MFT_REDUCE_MEAN, MFT_REDUCE_SUM, MFT_REDUCE_NONE = 0, 1, 2
 
@@ -111,6 +113,17 @@ class RmsNormDesc(C.Structure):
     _fields_ = [("N", C.c_int64), ("D", C.c_int64), ("dtype", C.c_int32), ("norm", C.c_int32), ("eps", C.c_float)] + \
         [(n, C.c_int64) for n in ("x_stride", "residual_stride", "total_stride", "y_stride", "dy_stride",
                                   "dtotal_stride", "dx_stride")]
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [("n", C.c_int64)] + [(n, C.c_void_p) for n in (
+        "param", "param_bf16", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")] + \
+        [("weight_decay", C.c_double)]
+
+
+class AdamWDesc(C.Structure):
+    _fields_ = [("lr", C.c_double), ("lr_device", C.c_void_p), ("beta1", C.c_double), ("beta2", C.c_double),
+                ("eps", C.c_double), ("max_norm", C.c_double), ("state_bits", C.c_int32)]
 
 
 class MftError(RuntimeError):
@@ -205,6 +218,10 @@ def lib():
     L.mft_rms_norm_workspace_size.argtypes = [C.POINTER(RmsNormDesc), C.POINTER(C.c_size_t)]
     L.mft_rms_norm_bwd.restype = C.c_int
     L.mft_rms_norm_bwd.argtypes = [C.POINTER(RmsNormDesc)] + [vp] * 9
+    L.mft_adamw_workspace_size.restype = C.c_int
+    L.mft_adamw_workspace_size.argtypes = [C.POINTER(AdamWDesc), C.c_int32, vp, C.POINTER(C.c_size_t)]
+    L.mft_adamw_step.restype = C.c_int
+    L.mft_adamw_step.argtypes = [C.POINTER(AdamWDesc), C.c_int32] + [vp] * 5
     if L.mft_version() != 7:
         raise RuntimeError("libmft_attn.so version mismatch")
     _lib = L
@@ -474,3 +491,18 @@ def rms_norm_workspace_size(d) -> int:
 
 def rms_norm_bwd(d, x, weight, rstd, dy, dtotal, dx, dweight, workspace, stream) -> None:
     check(lib().mft_rms_norm_bwd(C.byref(d), x, weight, rstd, dy, dtotal, dx, dweight, workspace, stream))
+
+
+def adamw_desc(lr, beta1=0.9, beta2=0.999, eps=1e-8, max_norm=0.0, state_bits=32, lr_device=None):
+    return AdamWDesc(lr, lr_device, beta1, beta2, eps, max_norm, state_bits)
+
+
+def adamw_workspace_size(d, tensors) -> int:
+    """tensors: a ctypes array of AdamWTensor, here and in adamw_step."""
+    n = C.c_size_t()
+    check(lib().mft_adamw_workspace_size(C.byref(d), len(tensors), tensors, C.byref(n)))
+    return n.value
+
+
+def adamw_step(d, tensors, step, norm, workspace, stream) -> None:
+    check(lib().mft_adamw_step(C.byref(d), len(tensors), tensors, step, norm, workspace, stream))
