@@ -1,0 +1,76 @@
+/*
+ * mft/gated_linear.h — C ABI of a gated linear layer on gfx950: the first half of
+ * a gated feed-forward block.
+ *
+ *   gate = x W_gate,  up = x W_up,  h = act(gate) * up
+ *
+ * x [N, in], W_gate and W_up [in, ff] or, with w_transposed, [ff, in]; h, gate and up
+ * [N, ff].  act is relu, the tanh form of GELU or SiLU, as mft/linear.h has them.
+ * Backward, with dgate = dh up act'(gate) and dup = dh act(gate):
+ *
+ *   dx = dgate W_gate^T + dup W_up^T,  dW_gate = x^T dgate,  dW_up = x^T dup
+ *
+ * All have element type `dtype`.  Products accumulate in fp32, and the activation and
+ * the product of both sums are applied to the accumulators: h, gate and up are
+ * rounded once.  With bf16, dgate and dup are rounded to bf16 for the matrix units
+ * (half a step of each product's operand, as x and W have), and dx and the
+ * weights' gradients once more where they are stored.  With fp32 the products are
+ * those of the LoRA layer's (csrc/gemm_f32.hip), and the forward's with one or two
+ * rows fp32 sums.  Results do not depend on the order in which workgroups run.
+ *
+ * In 8 bits x and the weights are e4m3 numbers (OCP) with one fp32 scale a row,
+ * as mft/rms_norm.h holds them, the weights [ff, in]:
+ *
+ *   gate(n, f) = x_scale(n) gate_scale(f) sum over k of x(n, k) W_gate(f, k),  up likewise
+ *
+ * summed in fp32, and h is bf16.  It is a forward only.
+ *
+ * Conventions are those of mft/linear.h: all operands contiguous, no allocation, N
+ * may be 0 (the weights' gradients are then zero); N of 2^31 or more, in and ff above
+ * 2^24, and products of more than 2^23 tiles of 64 x 64 are refused.
+ */
+#ifndef MFT_GATED_LINEAR_H
+#define MFT_GATED_LINEAR_H
+
+#include "mft/attention.h"
+#include "mft/linear.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+typedef struct {
+    int64_t N;             /* rows of x and h                                 */
+    int64_t in_dim;        /* columns of x                                    */
+    int64_t ff_dim;        /* columns of h                                    */
+    int32_t dtype;         /* MFT_F32 or MFT_BF16; MFT_BF16 (h's) in 8 bits   */
+    int32_t w_transposed;  /* W_gate and W_up stored [ff, in]; 1 in 8 bits    */
+    int32_t activation;    /* mft_activation, not MFT_ACT_NONE                */
+} mft_gated_linear_desc;
+
+/* Workspace bytes of the forward and backward (either may be 0). */
+mft_status mft_gated_linear_workspace_size(const mft_gated_linear_desc* desc, size_t* fwd_bytes, size_t* bwd_bytes);
+
+/* h, and gate and up (the backward's inputs) where they are not NULL: both or
+ * neither. */
+mft_status mft_gated_linear_fwd(const mft_gated_linear_desc* desc, const void* x, const void* W_gate, const void* W_up,
+                                void* h, void* gate, void* up, void* workspace, hipStream_t stream);
+
+/* dx, dW_gate and dW_up, each left out where NULL, written and not accumulated.  x
+ * may be NULL without the weights' gradients, the weights without dx. */
+mft_status mft_gated_linear_bwd(const mft_gated_linear_desc* desc, const void* x, const void* W_gate, const void* W_up,
+                                const void* gate, const void* up, const void* dh, void* dx, void* dW_gate, void* dW_up,
+                                void* workspace, hipStream_t stream);
+
+/* Workspace bytes of the forward in 8 bits. */
+mft_status mft_gated_linear_e4m3_workspace_size(const mft_gated_linear_desc* desc, size_t* bytes);
+
+/* h (bf16) from e4m3 numbers x [N, in], W_gate and W_up [ff, in] and their rows' scales. */
+mft_status mft_gated_linear_e4m3_fwd(const mft_gated_linear_desc* desc, const void* x, const float* x_scale,
+                                     const void* W_gate, const float* gate_scale, const void* W_up,
+                                     const float* up_scale, void* h, void* workspace, hipStream_t stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* MFT_GATED_LINEAR_H */

@@ -40,6 +40,8 @@ LAYER_EXPORTS = (
 # The same of the gated half of a block and its training step: rms_norm.h, gated_linear.h and adamw.h.
 BLOCK_EXPORTS = (
     "mft_rms_norm_fwd", "mft_rms_norm_e4m3_fwd", "mft_rms_norm_workspace_size", "mft_rms_norm_bwd",
+    "mft_gated_linear_workspace_size", "mft_gated_linear_fwd", "mft_gated_linear_bwd",
+    "mft_gated_linear_e4m3_workspace_size", "mft_gated_linear_e4m3_fwd",
     "mft_adamw_workspace_size", "mft_adamw_step",
 )
 LOGPROBS_MAX_TOP = 64
@@ -113,6 +115,11 @@ class RmsNormDesc(C.Structure):
     _fields_ = [("N", C.c_int64), ("D", C.c_int64), ("dtype", C.c_int32), ("norm", C.c_int32), ("eps", C.c_float)] + \
         [(n, C.c_int64) for n in ("x_stride", "residual_stride", "total_stride", "y_stride", "dy_stride",
                                   "dtotal_stride", "dx_stride")]
+
+
+class GatedLinearDesc(C.Structure):
+    _fields_ = [("N", C.c_int64), ("in_dim", C.c_int64), ("ff_dim", C.c_int64), ("dtype", C.c_int32),
+                ("w_transposed", C.c_int32), ("activation", C.c_int32)]
 
 
 class AdamWTensor(C.Structure):
@@ -218,6 +225,17 @@ def lib():
     L.mft_rms_norm_workspace_size.argtypes = [C.POINTER(RmsNormDesc), C.POINTER(C.c_size_t)]
     L.mft_rms_norm_bwd.restype = C.c_int
     L.mft_rms_norm_bwd.argtypes = [C.POINTER(RmsNormDesc)] + [vp] * 9
+    L.mft_gated_linear_workspace_size.restype = C.c_int
+    L.mft_gated_linear_workspace_size.argtypes = [C.POINTER(GatedLinearDesc), C.POINTER(C.c_size_t),
+                                                  C.POINTER(C.c_size_t)]
+    L.mft_gated_linear_fwd.restype = C.c_int
+    L.mft_gated_linear_fwd.argtypes = [C.POINTER(GatedLinearDesc)] + [vp] * 8
+    L.mft_gated_linear_bwd.restype = C.c_int
+    L.mft_gated_linear_bwd.argtypes = [C.POINTER(GatedLinearDesc)] + [vp] * 11
+    L.mft_gated_linear_e4m3_workspace_size.restype = C.c_int
+    L.mft_gated_linear_e4m3_workspace_size.argtypes = [C.POINTER(GatedLinearDesc), C.POINTER(C.c_size_t)]
+    L.mft_gated_linear_e4m3_fwd.restype = C.c_int
+    L.mft_gated_linear_e4m3_fwd.argtypes = [C.POINTER(GatedLinearDesc)] + [vp] * 9
     L.mft_adamw_workspace_size.restype = C.c_int
     L.mft_adamw_workspace_size.argtypes = [C.POINTER(AdamWDesc), C.c_int32, vp, C.POINTER(C.c_size_t)]
     L.mft_adamw_step.restype = C.c_int
@@ -491,6 +509,42 @@ def rms_norm_workspace_size(d) -> int:
 
 def rms_norm_bwd(d, x, weight, rstd, dy, dtotal, dx, dweight, workspace, stream) -> None:
     check(lib().mft_rms_norm_bwd(C.byref(d), x, weight, rstd, dy, dtotal, dx, dweight, workspace, stream))
+
+
+def gated_linear_desc(N, in_dim, ff_dim, dtype=MFT_F32, w_transposed=False, activation=MFT_ACT_GELU_TANH):
+    return GatedLinearDesc(N, in_dim, ff_dim, dtype, int(bool(w_transposed)), activation)
+
+
+def gated_linear_workspace_size(d):
+    f, b = C.c_size_t(), C.c_size_t()
+    check(lib().mft_gated_linear_workspace_size(C.byref(d), C.byref(f), C.byref(b)))
+    return f.value, b.value
+
+
+def gated_linear_fwd_workspace_size(d) -> int:
+    """The forward's alone: a call for its product need not plan the backward's."""
+    f = C.c_size_t()
+    check(lib().mft_gated_linear_workspace_size(C.byref(d), C.byref(f), None))
+    return f.value
+
+
+def gated_linear_fwd(d, x, W_gate, W_up, h, gate, up, workspace, stream) -> None:
+    check(lib().mft_gated_linear_fwd(C.byref(d), x, W_gate, W_up, h, gate, up, workspace, stream))
+
+
+def gated_linear_bwd(d, x, W_gate, W_up, gate, up, dh, dx, dW_gate, dW_up, workspace, stream) -> None:
+    check(lib().mft_gated_linear_bwd(C.byref(d), x, W_gate, W_up, gate, up, dh, dx, dW_gate, dW_up, workspace, stream))
+
+
+def gated_linear_e4m3_workspace_size(d) -> int:
+    n = C.c_size_t()
+    check(lib().mft_gated_linear_e4m3_workspace_size(C.byref(d), C.byref(n)))
+    return n.value
+
+
+def gated_linear_e4m3_fwd(d, x, x_scale, W_gate, gate_scale, W_up, up_scale, h, workspace, stream) -> None:
+    check(lib().mft_gated_linear_e4m3_fwd(C.byref(d), x, x_scale, W_gate, gate_scale, W_up, up_scale, h, workspace,
+                                          stream))
 
 
 def adamw_desc(lr, beta1=0.9, beta2=0.999, eps=1e-8, max_norm=0.0, state_bits=32, lr_device=None):

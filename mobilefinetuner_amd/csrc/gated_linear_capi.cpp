@@ -1,0 +1,250 @@
+// C ABI of the gated linear layer (declared in include/mft/gated_linear.h).
+#include "mft/gated_linear.h"
+
+#include <algorithm>
+#include <initializer_list>
+#include <string>
+
+#include "capi_util.h"
+#include "gemm_f32.h"
+#include "linear_kernels.h"
+
+namespace {
+
+using namespace mft::capi;
+
+size_t up(size_t x) { return (x + 255) & ~size_t(255); }
+
+mft_status check(const mft_gated_linear_desc* d, const char* who, bool e4m3 = false) {
+    if (!d) return fail(MFT_ERR_INVALID_ARG, std::string(who) + ": desc is NULL");
+    if (d->N < 0 || d->in_dim <= 0 || d->ff_dim <= 0)
+        return fail(MFT_ERR_INVALID_ARG, std::string(who) + ": x must be [N, in] and the weights [in, ff] with N >= 0 "
+                                                            "and positive dimensions");
+    if (d->N > (int64_t(1) << 31) - 1 || d->in_dim > (int64_t(1) << 24) || d->ff_dim > (int64_t(1) << 24))
+        return fail(MFT_ERR_UNSUPPORTED, std::string(who) + ": N must be below 2^31, in and ff at most 2^24");
+    if (e4m3 ? d->dtype != MFT_BF16 : d->dtype != MFT_F32 && d->dtype != MFT_BF16)
+        return fail(MFT_ERR_INVALID_ARG, std::string(who) + (e4m3 ? ": dtype (of h) must be MFT_BF16"
+                                                                  : ": dtype must be MFT_F32 or MFT_BF16"));
+    if (e4m3 && !d->w_transposed)
+        return fail(MFT_ERR_INVALID_ARG, std::string(who) + ": weights in 8 bits are stored [ff, in]");
+    if (d->activation <= MFT_ACT_NONE || d->activation > MFT_ACT_SILU)
+        return fail(MFT_ERR_INVALID_ARG, std::string(who) + ": activation must be RELU, GELU_TANH or SILU");
+    // a launch takes fewer than 2^32 threads: 2^23 tiles of at most 256
+    const int64_t n = (d->N + 63) / 64, i = (d->in_dim + 63) / 64, f = (d->ff_dim + 63) / 64;
+    if (std::max(n * f, std::max(n * i, i * f)) > (int64_t(1) << 23))
+        return fail(MFT_ERR_UNSUPPORTED, std::string(who) + ": N, in and ff are too large together");
+    return MFT_OK;
+}
+
+bool is_bf(const mft_gated_linear_desc* d) { return d->dtype == MFT_BF16; }
+// Columns of either half of dz: whole vectors in bf16.
+int64_t half_ld(const mft_gated_linear_desc* d) { return is_bf(d) ? (d->ff_dim + 7) / 8 * 8 : d->ff_dim; }
+
+mft::LinearProduct product_fwd(const mft_gated_linear_desc* d) {
+    mft::LinearProduct g{};
+    g.M = d->N, g.N = d->ff_dim, g.K = d->in_dim;
+    g.p_kc = 1, g.q_kc = d->w_transposed != 0;
+    g.act = d->activation;
+    return g;
+}
+mft::LinearProduct product_dx(const mft_gated_linear_desc* d) {  // along both halves of dz
+    mft::LinearProduct g{};
+    g.M = d->N, g.N = d->in_dim, g.K = g.ldp = 2 * half_ld(d);
+    g.joint = d->ff_dim;
+    g.p_kc = 1, g.q_kc = d->w_transposed == 0;
+    return g;
+}
+mft::LinearProduct product_dw(const mft_gated_linear_desc* d) {  // rows: the weight's first dimension
+    mft::LinearProduct g{};
+    g.M = d->w_transposed ? d->ff_dim : d->in_dim;
+    g.N = d->w_transposed ? d->in_dim : d->ff_dim;
+    g.K = d->N;
+    (d->w_transposed ? g.ldp : g.ldq) = 2 * half_ld(d);
+    return g;
+}
+mft::GemmF32 f_fwd(const mft_gated_linear_desc* d) {
+    mft::GemmF32 g{};
+    g.M = d->N, g.N = g.ldc = d->ff_dim;
+    g.terms[0] = {nullptr, nullptr, d->in_dim, d->w_transposed ? d->in_dim : d->ff_dim, d->in_dim, 0,
+                  d->w_transposed != 0, 1.f};
+    return g;
+}
+mft::GemmF32 f_dx(const mft_gated_linear_desc* d) {
+    mft::GemmF32 g{};
+    g.M = d->N, g.N = g.ldc = d->in_dim;
+    g.terms[0] = g.terms[1] = {nullptr, nullptr, 2 * d->ff_dim, d->w_transposed ? d->in_dim : d->ff_dim, d->ff_dim, 0,
+                               d->w_transposed == 0, 1.f};
+    return g;
+}
+mft::GemmF32 f_dw(const mft_gated_linear_desc* d) {
+    mft::GemmF32 g{};
+    g.M = d->w_transposed ? d->ff_dim : d->in_dim;
+    g.N = g.ldc = d->w_transposed ? d->in_dim : d->ff_dim;
+    g.terms[0] = {nullptr, nullptr, d->w_transposed ? 2 * d->ff_dim : d->in_dim,
+                  d->w_transposed ? d->in_dim : 2 * d->ff_dim, d->N, 1, 0, 1.f};
+    return g;
+}
+
+struct FwdLayout {
+    size_t gate, gemm, total;  // fp32: gate where the caller keeps none
+};
+FwdLayout fwd_layout(const mft_gated_linear_desc* d) {
+    FwdLayout l{};
+    const mft::LinearProduct g = product_fwd(d);
+    if (mft::few_rows(g)) return l;
+    if (is_bf(d)) {
+        l.total = mft::gated_gemm_workspace(g);
+        return l;
+    }
+    l.gemm = up((size_t)d->N * d->ff_dim * 4);
+    l.total = l.gemm + mft::gemm_f32_workspace(f_fwd(d));
+    return l;
+}
+struct BwdLayout {
+    size_t dz, gemm, total;
+};
+BwdLayout bwd_layout(const mft_gated_linear_desc* d) {
+    BwdLayout l{};
+    l.gemm = up((size_t)d->N * 2 * half_ld(d) * (is_bf(d) ? 2 : 4));
+    l.total = l.gemm + (is_bf(d) ? std::max(mft::joined_gemm_workspace(product_dx(d)), mft::bf_gemm_workspace(product_dw(d)))
+                                 : std::max(mft::gemm_f32_workspace(f_dx(d)), mft::gemm_f32_workspace(f_dw(d))));
+    return l;
+}
+
+bool any_is(const void* p, std::initializer_list<const void*> of) {
+    return p && std::find(of.begin(), of.end(), p) != of.end();
+}
+
+}  // namespace
+
+extern "C" {
+
+mft_status mft_gated_linear_workspace_size(const mft_gated_linear_desc* desc, size_t* fwd_bytes, size_t* bwd_bytes) {
+    const mft_status r = check(desc, "mft_gated_linear_workspace_size");
+    if (r != MFT_OK) return r;
+    const bool empty = desc->N == 0;
+    if (fwd_bytes) *fwd_bytes = empty ? 0 : fwd_layout(desc).total;
+    if (bwd_bytes) *bwd_bytes = empty ? 0 : bwd_layout(desc).total;
+    return MFT_OK;
+}
+
+mft_status mft_gated_linear_fwd(const mft_gated_linear_desc* desc, const void* x, const void* W_gate, const void* W_up,
+                                void* h, void* gate, void* up, void* workspace, hipStream_t stream) {
+    const char* who = "mft_gated_linear_fwd";
+    const mft_status r = check(desc, who);
+    if (r != MFT_OK) return r;
+    if (desc->N == 0) return MFT_OK;
+    if (!x || !W_gate || !W_up || !h)
+        return fail(MFT_ERR_INVALID_ARG, "mft_gated_linear_fwd: x, W_gate, W_up and h must be non-NULL");
+    if (!gate != !up) return fail(MFT_ERR_INVALID_ARG, "mft_gated_linear_fwd: gate and up are kept together");
+    if (any_is(h, {x, W_gate, W_up, gate, up}) || any_is(gate, {x, W_gate, W_up, up}) || any_is(up, {x, W_gate, W_up}))
+        return fail(MFT_ERR_INVALID_ARG, "mft_gated_linear_fwd: h, gate and up may not be one another or operands");
+    const FwdLayout l = fwd_layout(desc);
+    char* ws = static_cast<char*>(workspace);
+    if (!ws && l.total > 0) return fail(MFT_ERR_INVALID_ARG, "mft_gated_linear_fwd: workspace must be non-NULL");
+    mft::LinearProduct q = product_fwd(desc);
+    q.P = x;
+    q.Q = W_gate;
+    q.Q2 = W_up;
+    q.C = h;
+    q.z = gate;
+    q.z2 = up;
+    q.partial = reinterpret_cast<float*>(ws);
+    if (mft::few_rows(q)) return hip_status(mft::launch_gated_rows(q, is_bf(desc), stream), "mft_gated_linear_fwd launch");
+    if (is_bf(desc)) return hip_status(mft::launch_gated_gemm(q, stream), "mft_gated_linear_fwd launch");
+    mft::GemmF32 g = f_fwd(desc);
+    float* first = gate ? static_cast<float*>(gate) : reinterpret_cast<float*>(ws + l.gate);
+    g.partial = reinterpret_cast<float*>(ws + l.gemm);
+    g.terms[0].A = static_cast<const float*>(x);
+    g.terms[0].B = static_cast<const float*>(W_gate);
+    g.C = first;
+    hipError_t e = mft::launch_gemm_f32(g, stream);
+    g.terms[0].B = static_cast<const float*>(W_up);
+    g.C = static_cast<float*>(h);
+    g.z = static_cast<float*>(up);
+    g.gate = first;
+    g.act = desc->activation;
+    if (e == hipSuccess) e = mft::launch_gemm_f32(g, stream);
+    return hip_status(e, "mft_gated_linear_fwd launch");
+}
+
+mft_status mft_gated_linear_bwd(const mft_gated_linear_desc* desc, const void* x, const void* W_gate, const void* W_up,
+                                const void* gate, const void* up, const void* dh, void* dx, void* dW_gate, void* dW_up,
+                                void* workspace, hipStream_t stream) {
+    const char* who = "mft_gated_linear_bwd";
+    const mft_status r = check(desc, who);
+    if (r != MFT_OK) return r;
+    const bool bf = is_bf(desc);
+    void* const dW[2] = {dW_gate, dW_up};
+    hipError_t e = hipSuccess;
+    if (desc->N == 0) {
+        for (void* w : dW)
+            if (w && e == hipSuccess) e = mft::launch_fill_zero(w, (size_t)desc->in_dim * desc->ff_dim * (bf ? 2 : 4), stream);
+        return hip_status(e, "mft_gated_linear_bwd launch");
+    }
+    if (!dx && !dW_gate && !dW_up) return MFT_OK;
+    if (!gate || !up || !dh || !workspace || ((dW_gate || dW_up) && !x) || (dx && (!W_gate || !W_up)))
+        return fail(MFT_ERR_INVALID_ARG, "mft_gated_linear_bwd: gate, up, dh, workspace, x (for the weights' gradients) "
+                                         "and the weights (for dx) must be non-NULL");
+    for (void* o : {dx, dW_gate, dW_up})
+        if (any_is(o, {x, W_gate, W_up, gate, up, dh}))
+            return fail(MFT_ERR_INVALID_ARG, "mft_gated_linear_bwd: a gradient may not be an operand");
+    if (any_is(dx, {dW_gate, dW_up}) || any_is(dW_gate, {dW_up}))
+        return fail(MFT_ERR_INVALID_ARG, "mft_gated_linear_bwd: the gradients may not be one another");
+    const BwdLayout l = bwd_layout(desc);
+    char* ws = static_cast<char*>(workspace);
+    const int64_t ld = half_ld(desc);
+    float* sums = reinterpret_cast<float*>(ws + l.gemm);
+    const char* dz[2] = {ws + l.dz, ws + l.dz + ld * (bf ? 2 : 4)};
+    e = mft::launch_gated_dz(gate, up, dh, ws + l.dz, desc->N, desc->ff_dim, ld, desc->activation, bf, stream);
+    if (e == hipSuccess && dx) {
+        if (bf) {
+            mft::LinearProduct g = product_dx(desc);
+            g.P = dz[0], g.Q = W_gate, g.Q2 = W_up, g.C = dx, g.partial = sums;
+            e = mft::launch_joined_gemm(g, stream);
+        } else {
+            mft::GemmF32 g = f_dx(desc);
+            for (int i = 0; i < 2; ++i) {
+                g.terms[i].A = reinterpret_cast<const float*>(dz[i]);
+                g.terms[i].B = static_cast<const float*>(i ? W_up : W_gate);
+            }
+            g.C = static_cast<float*>(dx), g.partial = sums;
+            e = mft::launch_gemm_f32(g, stream);
+        }
+    }
+    for (int i = 0; i < 2 && e == hipSuccess; ++i) {
+        if (!dW[i]) continue;
+        const void* rows = desc->w_transposed ? dz[i] : x;
+        const void* cols = desc->w_transposed ? x : dz[i];
+        if (bf) {
+            mft::LinearProduct g = product_dw(desc);
+            g.P = rows, g.Q = cols, g.C = dW[i], g.partial = sums;
+            e = mft::launch_bf_gemm(g, stream);
+        } else {
+            mft::GemmF32 g = f_dw(desc);
+            g.terms[0].A = static_cast<const float*>(rows), g.terms[0].B = static_cast<const float*>(cols);
+            g.C = static_cast<float*>(dW[i]), g.partial = sums;
+            e = mft::launch_gemm_f32(g, stream);
+        }
+    }
+    return hip_status(e, "mft_gated_linear_bwd launch");
+}
+
+mft_status mft_gated_linear_e4m3_workspace_size(const mft_gated_linear_desc* desc, size_t* bytes) {
+    const mft_status r = check(desc, "mft_gated_linear_e4m3_workspace_size", true);
+    if (r != MFT_OK) return r;
+    if (bytes) *bytes = 0;
+    return MFT_OK;
+}
+
+mft_status mft_gated_linear_e4m3_fwd(const mft_gated_linear_desc* desc, const void* x, const float* x_scale,
+                                     const void* W_gate, const float* gate_scale, const void* W_up,
+                                     const float* up_scale, void* h, void* workspace, hipStream_t stream) {
+    const char* who = "mft_gated_linear_e4m3_fwd";
+    const mft_status r = check(desc, who, true);
+    if (r != MFT_OK) return r;
+    (void)x_scale, (void)gate_scale, (void)up_scale, (void)x, (void)W_gate, (void)W_up, (void)h, (void)workspace, (void)stream;
+    return fail(MFT_ERR_UNSUPPORTED, "mft_gated_linear_e4m3_fwd: not built");
+}
+
+}  // extern "C"

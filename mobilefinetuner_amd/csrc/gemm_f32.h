@@ -33,6 +33,8 @@ struct GemmF32 {
     int act;
     const float* residual;
     float* z;
+    // The gated linear layer's, with the same: z is the sum, C = act(gate) times it; no bias or residual.
+    const float* gate;  // [M, N] or null
 };
 
 // Workspace bytes: fp32 partial products where K is split across workgroups.

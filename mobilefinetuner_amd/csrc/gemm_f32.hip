@@ -186,8 +186,17 @@ struct Doubt {
     __device__ __forceinline__ bool any() const { return least < ((127u - 80u) << 24) - 1u || sum != sum; }
 };
 
-// The linear layer's epilogue of VEC columns n of row m (GemmF32).
+// The linear layer's epilogue of VEC columns n of row m (GemmF32), or the gated one's.
 template <int VEC> __device__ __forceinline__ void run_epilogue(const GemmF32& g, int64_t m, int64_t n, float* v) {
+    if (g.gate) {
+        float gate[VEC];
+        if (g.z) store_part<float, VEC>(g.z + m * g.N, n, g.N, v);
+        load_part<float, VEC>(g.gate + m * g.N, n, g.N, gate);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] *= act_value_of(g.act, gate[e]);
+        store_part<float, VEC>(g.C + m * g.N, n, g.N, v);
+        return;
+    }
     LinearProduct p{};
     p.N = g.N;
     p.C = g.C;
@@ -590,7 +599,7 @@ Plan plan(const GemmF32& g) {
     return p;
 }
 
-bool with_epilogue(const GemmF32& g) { return g.act != ACT_NONE || g.residual || g.z; }
+bool with_epilogue(const GemmF32& g) { return g.act != ACT_NONE || g.residual || g.z || g.gate; }
 
 template <int T, int BK, int KW>
 void launch_t(const Args& a, hipStream_t st) {

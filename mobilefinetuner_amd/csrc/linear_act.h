@@ -40,4 +40,12 @@ template <int ACT> __device__ __forceinline__ float act_grad(float z) {
     return 1.f;
 }
 
+// The same by an activation that a launch's threads share.
+__device__ __forceinline__ float act_value_of(int act, float z) {
+    return act == ACT_GELU_TANH ? act_value<ACT_GELU_TANH>(z) : act == ACT_SILU ? act_value<ACT_SILU>(z) : act_value<ACT_RELU>(z);
+}
+__device__ __forceinline__ float act_grad_of(int act, float z) {
+    return act == ACT_GELU_TANH ? act_grad<ACT_GELU_TANH>(z) : act == ACT_SILU ? act_grad<ACT_SILU>(z) : act_grad<ACT_RELU>(z);
+}
+
 }  // namespace mft

@@ -1,5 +1,6 @@
 // Launchers of the linear layer's kernels (linear_gemm.hip, linear_rows.hip,
-// linear.hip; called by linear_capi.cpp).
+// linear.hip; called by linear_capi.cpp) and of the gated linear layer's
+// (gated_gemm.hip, gated_rows.hip, gated.hip; called by gated_linear_capi.cpp).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -27,6 +28,11 @@ struct LinearProduct {
     void* z;               // [M, N], before the activation, or null
     int act;
     float* partial;        // workspace of bf_gemm_workspace bytes
+    // A second Q, stored as the first: of the gated product C = act(P Q^T) (P Q2^T), with z the first
+    // sum and z2 the second, both or neither; or of a product joined along k, from `joint` on.
+    const void* Q2;
+    void* z2;
+    int64_t joint;
 };
 // bf16, any sizes (linear_gemm.hip).
 size_t bf_gemm_workspace(const LinearProduct& g);
@@ -34,6 +40,20 @@ hipError_t launch_bf_gemm(const LinearProduct& g, hipStream_t st);
 // Few rows with p_kc (linear_rows.hip); no workspace.
 bool few_rows(const LinearProduct& g);
 hipError_t launch_few_rows(const LinearProduct& g, bool bf16, hipStream_t st);
+
+// The gated product in bf16, any sizes (gated_gemm.hip): no bias, no residual.
+size_t gated_gemm_workspace(const LinearProduct& g);
+hipError_t launch_gated_gemm(const LinearProduct& g, hipStream_t st);
+// sum_k P(m, k) Q(n, k) over k < joint plus the sum over the rest with Q2, P of rows of ldp elements: Q and Q2
+// hold `joint` k each and K = 2 joint (gated_gemm.hip).
+size_t joined_gemm_workspace(const LinearProduct& g);
+hipError_t launch_joined_gemm(const LinearProduct& g, hipStream_t st);
+// Few rows (gated_rows.hip); no workspace.
+hipError_t launch_gated_rows(const LinearProduct& g, bool bf16, hipStream_t st);
+// dz[N, 2 ld] = (dh up act'(gate) | dh act(gate)), either half padded with zeros from ff to ld columns
+// (gated.hip).
+hipError_t launch_gated_dz(const void* gate, const void* up, const void* dh, void* dz, int64_t N, int64_t ff, int64_t ld,
+                           int act, bool bf16, hipStream_t st);
 
 // dz = dy act'(z) ([N, out]; no act: dz is not written) and db[out] = the sums
 // of dz's columns before rounding (null: left out).

@@ -1,0 +1,382 @@
+"""The gated linear layer (mft_gated_linear_* through the torch helpers) against its
+formulas in 64 bits, and refusals.
+
+Bounds, per element, with u = 2^-24 and h half a step of the type (2^-8 for bf16).
+gate and up are products of K terms in fp32: off by 2 (K + 8) u of the sum of the
+magnitudes (the products of bf16 and of e4m3 numbers are exact; twice over in case
+the matrix unit truncates), and stored by h of themselves more.  The activations'
+slopes stay under 1.13, and their own evaluation under u (24 + 8 |z|) of max(|y|,
+|z|).  The backward is given gate and up: act'(z) is off by u (32 + 16 |z|^2 + 16 |z|);
+dgate and dup, rounded to bf16, by h of themselves more; dx and the weights' gradients
+carry that through their sums.
+"""
+import ctypes as C
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+U = 2.0 ** -24
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+ACTS = {"relu": F.relu, "gelu_tanh": lambda z: F.gelu(z, approximate="tanh"), "silu": F.silu}
+
+
+def half(t):
+    return torch.finfo(t).eps / 2 if t == torch.bfloat16 else U
+
+
+def make(N, n_in, n_ff, dtype, seed, w_t=False):
+    g = torch.Generator().manual_seed(seed)
+    t = DT[dtype]
+    x = torch.randn(N, n_in, generator=g).to(t)
+    Wg, Wu = ((torch.randn(n_in, n_ff, generator=g) / math.sqrt(n_in)).to(t) for _ in range(2))
+    gate, up = ((1.5 * torch.randn(N, n_ff, generator=g)).to(t) for _ in range(2))
+    dh = (0.1 * torch.randn(N, n_ff, generator=g)).to(t)
+    return dict(x=x, W_gate=Wg.t().contiguous() if w_t else Wg, W_up=Wu.t().contiguous() if w_t else Wu, gate=gate, up=up,
+                dh=dh)
+
+
+def of_act(z, act):
+    """act(z), and how far the kernels' may be off it."""
+    y = ACTS[act](z)
+    return y, U * (24 + 8 * z.abs()) * torch.maximum(y.abs(), z.abs()) if act != "relu" else torch.zeros_like(y)
+
+
+def ref_forward(x, Wg, Wu, act, t, scale=(1.0, 1.0, 1.0)):
+    """(gate, its bound, up, its bound, h, its bound), W [in, ff] in 64 bits, times the rows' scales."""
+    K = x.shape[1]
+    xs, gs, us = scale
+    out = []
+    for W, s in ((Wg, gs), (Wu, us)):
+        z = (x @ W) * xs * s
+        out.append((z, 2 * (K + 8) * U * (x.abs() @ W.abs()) * xs * s + 4 * U * z.abs()))
+    (g, eg), (u, eu) = out
+    a, ea = of_act(g, act)
+    h = a * u
+    eh = u.abs() * (1.13 * eg + ea) + a.abs() * eu + (1.13 * eg + ea) * eu + (half(t) + 2 * U) * h.abs() + 1e-30
+    return g, eg + half(t) * g.abs() + 1e-30, u, eu + half(t) * u.abs() + 1e-30, h, eh
+
+
+def ref_backward(x, Wg, Wu, gate, up, dh, act, t):
+    z = gate.clone().requires_grad_(True)
+    slope, = torch.autograd.grad(ACTS[act](z).sum(), z)
+    a, ea = of_act(gate, act)
+    dg, du = dh * up * slope, dh * a
+    h = half(t) if t == torch.bfloat16 else 0
+    es = 0 if act == "relu" else U * (32 + 16 * gate * gate + 16 * gate.abs())
+    eg = (dh * up).abs() * es + (4 * U + h) * dg.abs()
+    eu = dh.abs() * ea + (2 * U + h) * du.abs()
+    N, ff = dg.shape
+    dx = dg @ Wg.t() + du @ Wu.t()
+    mags = dg.abs() @ Wg.abs().t() + du.abs() @ Wu.abs().t()
+    ex = eg @ Wg.abs().t() + eu @ Wu.abs().t() + 2 * (2 * ff + 16) * U * mags + half(t) * dx.abs() + 1e-30
+    out = [dx, ex]
+    for d, e in ((dg, eg), (du, eu)):
+        dW = x.t() @ d
+        out += [dW, x.abs().t() @ e + 2 * (N + 8) * U * (x.abs().t() @ d.abs()) + half(t) * dW.abs() + 1e-30]
+    return out
+
+
+def within(got, ref, tol, what=""):
+    assert got.shape == ref.shape
+    off = (got.detach().double() - ref).abs()
+    worst = float((off / tol).max()) if off.numel() else 0.0
+    assert worst <= 1.0, f"{what}: {worst:.3g} times the bound"
+
+
+def check(dev, N, n_in, n_ff, dtype, act, w_t, seed):
+    from mobilefinetuner_amd import gated_linear as L
+    print(f"[case] {N} x {n_in} -> {n_ff} {dtype} {act} {'[ff, in]' if w_t else '[in, ff]'}", flush=True)
+    d = {k: v.to(dev) for k, v in make(N, n_in, n_ff, dtype, seed, w_t).items()}
+    up = {k: v.double() for k, v in d.items()}
+    Wg, Wu = (up[k].t() if w_t else up[k] for k in ("W_gate", "W_up"))
+    t = DT[dtype]
+    h, gate, rise = L.gated_linear(d["x"], d["W_gate"], d["W_up"], act, w_t, want_preact=True)
+    rg, tg, ru, tu, rh, th = ref_forward(up["x"], Wg, Wu, act, t)
+    assert h.dtype == gate.dtype == rise.dtype == t
+    within(gate, rg, tg, "gate")
+    within(rise, ru, tu, "up")
+    within(h, rh, th, "h")
+    only = L.gated_linear(d["x"], d["W_gate"], d["W_up"], act, w_t)
+    assert torch.equal(only[0], h) and only[1] is None and only[2] is None
+    dx, dWg, dWu = L.gated_linear_backward(d["x"], d["W_gate"], d["W_up"], d["gate"], d["up"], d["dh"], act, w_t)
+    rx, tx, rwg, twg, rwu, twu = ref_backward(up["x"], Wg, Wu, up["gate"], up["up"], up["dh"], act, t)
+    if w_t:
+        rwg, twg, rwu, twu = rwg.t(), twg.t(), rwu.t(), twu.t()
+    assert dx.dtype == dWg.dtype == dWu.dtype == t
+    within(dx, rx, tx, "dx")
+    within(dWg, rwg, twg, "dW_gate")
+    within(dWu, rwu, twu, "dW_up")
+
+
+# N, in, ff: one token and few, each tile with whole and ragged edges, odd sizes, K below a stage and
+# with a partial last stage, sizes of one
+SHAPES = [(1, 1, 1), (1, 64, 64), (1, 768, 1024), (1, 33, 4100), (2, 1024, 512), (2, 100, 9), (3, 33, 17), (5, 640, 2048),
+          (8, 896, 896), (17, 65, 130), (33, 128, 64), (64, 64, 64), (100, 200, 300), (129, 257, 511), (128, 128, 256),
+          (300, 1152, 640), (333, 72, 1000), (1000, 8, 8), (1024, 512, 256), (513, 1000, 104)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("w_t", [False, True], ids=["in_ff", "ff_in"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_forward_and_backward(dev, shape, dtype, w_t):
+    check(dev, *shape, dtype, "gelu_tanh", w_t, sum(shape))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 200, 72), (3, 200, 136), (150, 96, 264)], ids=lambda s: "x".join(map(str, s)))
+def test_activations(dev, shape, dtype, act):
+    for w_t in (False, True):
+        check(dev, *shape, dtype, act, w_t, 7)
+
+
+# products that fill the GPU with the largest tiles, with the middle ones, and that are cut along K; off 16
+# bytes with and without copies
+@pytest.mark.gpu
+@pytest.mark.parametrize("w_t", [False, True], ids=["in_ff", "ff_in"])
+@pytest.mark.parametrize("shape", [(4096, 256, 2048), (4100, 264, 2056), (2048, 320, 1024), (96, 4096, 128),
+                                   (2000, 2048, 72), (512, 1024, 8192), (700, 1153, 2001), (2000, 601, 1999),
+                                   (256, 2048, 1024), (64, 8192, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_large_products(dev, shape, w_t):
+    check(dev, *shape, "bf16", "silu", w_t, 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_leading_dimensions_and_other_layouts(dev, dtype):
+    """Batches of rows, operands that are not contiguous and weights off 16 bytes: the results of copies."""
+    from mobilefinetuner_amd import gated_linear as L
+    d = {k: v.to(dev) for k, v in make(24, 96, 136, dtype, 5).items()}
+    call = lambda x, a, b: L.gated_linear(x, a, b, "silu", False, True)  # noqa: E731
+    ref = call(d["x"], d["W_gate"], d["W_up"])
+    got = call(d["x"].view(2, 3, 4, 96), d["W_gate"], d["W_up"])
+    assert got[0].shape == (2, 3, 4, 136) and all(torch.equal(p.view(24, 136), q) for p, q in zip(got, ref))
+
+    def shifted(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=dev)[1:]
+        return flat.view(t.shape).copy_(t)
+
+    wide = torch.zeros(24, 200, dtype=DT[dtype], device=dev)
+    wide[:, 7:103] = d["x"]
+    for x, a, b in ((wide[:, 7:103], d["W_gate"].t().contiguous().t(), d["W_up"]),
+                    (shifted(d["x"]), d["W_gate"], shifted(d["W_up"])), (d["x"], shifted(d["W_gate"]), d["W_up"])):
+        for p, q in zip(call(x, a, b), ref):
+            assert torch.equal(p, q) or float((p - q).abs().max()) <= 2 * half(DT[dtype]) * float(q.abs().max())
+    back = L.gated_linear_backward(d["x"], d["W_gate"], d["W_up"], d["gate"], d["up"], d["dh"], "silu")
+    other = L.gated_linear_backward(d["x"].view(4, 6, 96), shifted(d["W_gate"]), shifted(d["W_up"]),
+                                    d["gate"].view(4, 6, 136), d["up"].view(4, 6, 136), d["dh"].view(4, 6, 136), "silu")
+    for p, q in zip(other, back):
+        assert float((p.view(q.shape) - q).abs().max()) <= 2 * half(DT[dtype]) * float(q.abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_no_rows_and_parts_of_the_gradient(dev, dtype):
+    from mobilefinetuner_amd import gated_linear as L
+    for N in (0, 40):
+        d = {k: v.to(dev) for k, v in make(N, 72, 48, dtype, 6).items()}
+        args = [d[k] for k in ("x", "W_gate", "W_up", "gate", "up", "dh")]
+        assert L.gated_linear(*args[:3])[0].shape == (N, 48)
+        whole = L.gated_linear_backward(*args)
+        if N == 0:
+            assert whole[0].shape == (0, 72) and (whole[1] == 0).all() and (whole[2] == 0).all()
+        for want in ((True, False, False), (False, True, False), (False, False, True), (False, False, False)):
+            only = L.gated_linear_backward(*args, want_x=want[0], want_gate=want[1], want_up=want[2])
+            for o, w, on in zip(only, whole, want):
+                assert torch.equal(o, w) if on else o is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("w_t", [False, True])
+def test_values_that_are_not_numbers(dev, w_t):
+    """A NaN of x stays in its row, one of a weight in its column."""
+    from mobilefinetuner_amd import gated_linear as L
+    for dtype in ("f32", "bf16"):
+        for N in (1, 70):
+            d = {k: v.to(dev) for k, v in make(N, 136, 200, dtype, 9, w_t).items()}
+            clean = L.gated_linear(d["x"], d["W_gate"], d["W_up"], "silu", w_t)[0]
+            x, W = d["x"].clone(), d["W_up"].clone()
+            x[N // 2, 5] = math.nan
+            h = L.gated_linear(x, d["W_gate"], d["W_up"], "silu", w_t)[0]
+            rows = torch.arange(N, device=dev) != N // 2
+            assert torch.isnan(h[N // 2]).all() and torch.equal(h[rows], clean[rows])
+            W[(33, 7) if w_t else (7, 33)] = math.nan
+            h = L.gated_linear(d["x"], d["W_gate"], W, "silu", w_t)[0]
+            cols = torch.arange(200, device=dev) != 33
+            assert torch.isnan(h[:, 33]).all() and torch.equal(h[:, cols], clean[:, cols])
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(dev):
+    """More than 2^31 values of h: the last rows are those of a call of their own, to the rounding of h."""
+    from mobilefinetuner_amd import gated_linear as L
+    N, n_in, n_ff = (1 << 18) + 40, 64, 8320
+    d = {k: v.to(dev) for k, v in make(40, n_in, n_ff, "bf16", 11).items()}
+    x = torch.zeros(N, n_in, dtype=torch.bfloat16, device=dev)
+    x[-40:] = d["x"]
+    h, gate, up = L.gated_linear(x, d["W_gate"], d["W_up"], "silu", False, True)
+    ref = L.gated_linear(d["x"], d["W_gate"], d["W_up"], "silu", False, True)
+    for p, q in zip((h, gate, up), ref):
+        assert float((p[-40:] - q).abs().max()) <= 2 * half(torch.bfloat16) * float(q.abs().max())
+        assert (p[:100] == 0).all()
+    gate[-40:], up[-40:] = d["gate"], d["up"]
+    h[-40:] = d["dh"]
+    dx, dWg, dWu = L.gated_linear_backward(x, d["W_gate"], d["W_up"], gate, up, h, "silu")
+    back = L.gated_linear_backward(d["x"], d["W_gate"], d["W_up"], d["gate"], d["up"], d["dh"], "silu")
+    assert (dx[:100] == 0).all()
+    for p, q in zip((dx[-40:], dWg, dWu), back):
+        assert float((p - q).abs().max()) <= 2 * half(torch.bfloat16) * float(q.abs().max())
+    del h, gate, up
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("act", list(ACTS))
+def test_autograd_gradients_against_differences(dev, dtype, act):
+    """The node's gradients are the helpers', and (fp32) those of differences: the loss sum(h c) moves by the
+    gradient along a direction v, to the second order of the step and the loss's rounding over it.  ReLU has
+    no second order where gate's sign stays: its gates are kept from zero."""
+    from mobilefinetuner_amd import gated_linear as L
+    s = {k: v.to(dev) for k, v in make(7, 40, 24, dtype, 8).items()}
+    leaves = [s[k].clone().requires_grad_(True) for k in ("x", "W_gate", "W_up")]
+    h = L.GatedLinear.apply(*leaves, act, False)
+    h.backward(s["dh"])
+    at = [v.detach() for v in leaves]
+    _, gate, up = L.gated_linear(*at, act, False, True)
+    for g, r in zip((v.grad for v in leaves), L.gated_linear_backward(*at, gate, up, s["dh"], act)):
+        assert torch.equal(g, r)
+    if dtype == "bf16" or act == "relu":
+        return
+    g = torch.Generator().manual_seed(1)
+    t = 2.0 ** -7
+    for i, p in enumerate(at):
+        v = torch.randn(p.shape, generator=g).to(dev) * (1.0 if i == 0 else 40 ** -0.5)
+        loss = []
+        for k in (t, -t):
+            q = [u + k * v if j == i else u for j, u in enumerate(at)]
+            loss.append(float((L.gated_linear(*q, act)[0].double() * s["dh"].double()).sum()))
+        slope = (loss[0] - loss[1]) / (2 * t)
+        scale = float(s["dh"].double().norm() * v.double().norm()) * math.sqrt(24) * 4
+        assert abs(slope - float((leaves[i].grad.double() * v.double()).sum())) <= scale * (4 * t * t + 256 * U / t)
+
+
+@pytest.mark.gpu
+def test_repeated_calls_and_streams(dev):
+    """The same bits from every call, also from two streams at once, each with its own workspace."""
+    from mobilefinetuner_amd import gated_linear as L
+    for shape in ((600, 512, 384), (96, 4096, 128)):
+        d = {k: v.to(dev) for k, v in make(*shape, "bf16", 9).items()}
+        args = [d[k] for k in ("x", "W_gate", "W_up", "gate", "up", "dh")]
+        ref = L.gated_linear(*args[:3])[:1] + L.gated_linear_backward(*args)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = []
+        for i in range(6):
+            with torch.cuda.stream(streams[i % 2]):
+                got.append(L.gated_linear(*args[:3])[:1] + L.gated_linear_backward(*args))
+        torch.cuda.synchronize()
+        for r in got:
+            assert all(torch.equal(p, q) for p, q in zip(r, ref))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_captured_graph_follows_its_inputs(dev, dtype):
+    from mobilefinetuner_amd import gated_linear as L
+    names = ("x", "W_gate", "W_up", "gate", "up", "dh")
+    d = {k: v.to(dev) for k, v in make(96, 1024, 136, dtype, 10).items()}
+
+    def step():
+        return L.gated_linear(*(d[k] for k in names[:3]))[:1] + L.gated_linear_backward(*(d[k] for k in names))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in (11, 12, 13):
+        for k, v in make(96, 1024, 136, dtype, seed).items():
+            d[k].copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(held, step()))
+
+
+# ------------------------------------------------------------------ refusals
+@pytest.fixture(scope="module")
+def capi():
+    from mobilefinetuner_amd import capi as M
+    M.lib()
+    return M
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(N=-1), "N >= 0"), (dict(in_dim=0), "positive"), (dict(ff_dim=0), "positive"), (dict(N=1 << 31), "below"),
+    (dict(in_dim=(1 << 24) + 1), "at most"), (dict(ff_dim=(1 << 24) + 1), "at most"), (dict(dtype=1), "dtype"),
+    (dict(activation=0), "activation"), (dict(activation=4), "activation"),
+    (dict(N=1 << 24, ff_dim=1 << 20), "too large together"),
+])
+def test_descriptors_refused(capi, change, message):
+    d = capi.gated_linear_desc(**{**dict(N=4, in_dim=64, ff_dim=32, dtype=capi.MFT_BF16, w_transposed=True), **change})
+    with pytest.raises(capi.MftError, match=message):
+        capi.gated_linear_workspace_size(d)
+    with pytest.raises(capi.MftError, match=message):
+        capi.gated_linear_fwd(d, 16, 32, 48, 64, None, None, 80, None)
+    with pytest.raises(capi.MftError, match=message):
+        capi.gated_linear_bwd(d, 16, 32, 48, 64, 80, 96, 112, 128, 144, 160, None)
+    with pytest.raises(capi.MftError, match=message):
+        capi.gated_linear_e4m3_workspace_size(d)
+    with pytest.raises(capi.MftError, match=message):
+        capi.gated_linear_e4m3_fwd(d, 16, 32, 48, 64, 80, 96, 112, 128, None)
+
+
+def test_operands_refused(capi):
+    d = capi.gated_linear_desc(4, 64, 32)
+    fwd, bwd = [16, 32, 48, 64, 80, 96, 112], [16, 32, 48, 64, 80, 96, 112, 128, 144, 160]
+    but = lambda a, **c: [c.get(f"_{i}", v) for i, v in enumerate(a)]  # noqa: E731
+    for i in (0, 1, 2, 3, 6):
+        with pytest.raises(capi.MftError, match="non-NULL"):
+            capi.gated_linear_fwd(d, *but(fwd, **{f"_{i}": None}), None)
+    for i in (4, 5):
+        with pytest.raises(capi.MftError, match="together"):
+            capi.gated_linear_fwd(d, *but(fwd, **{f"_{i}": None}), None)
+    for i, j in ((3, 0), (3, 1), (3, 2), (3, 4), (3, 5), (4, 0), (4, 5), (5, 2)):
+        with pytest.raises(capi.MftError, match="may not be"):
+            capi.gated_linear_fwd(d, *but(fwd, **{f"_{i}": fwd[j]}), None)
+    for i in (0, 1, 2, 3, 4, 5, 9):
+        with pytest.raises(capi.MftError, match="non-NULL"):
+            capi.gated_linear_bwd(d, *but(bwd, **{f"_{i}": None}), None)
+    for i, j in ((6, 5), (6, 0), (7, 1), (8, 3), (6, 7), (6, 8), (7, 8)):
+        with pytest.raises(capi.MftError, match="may not be"):
+            capi.gated_linear_bwd(d, *but(bwd, **{f"_{i}": bwd[j]}), None)
+    assert capi.lib().mft_gated_linear_fwd(None, *fwd, None) == capi.MFT_ERR_INVALID_ARG
+    empty = C.byref(capi.gated_linear_desc(0, 64, 32))
+    assert capi.lib().mft_gated_linear_fwd(empty, *[None] * 8) == capi.MFT_OK
+    assert capi.lib().mft_gated_linear_bwd(empty, *[None] * 11) == capi.MFT_OK
+
+
+def test_no_cpu_path():
+    from mobilefinetuner_amd import gated_linear as L
+    with pytest.raises(ValueError, match="no CPU path"):
+        L.gated_linear(torch.zeros(2, 4), torch.zeros(4, 3), torch.zeros(4, 3))
+
+
+@pytest.mark.gpu
+def test_operands_that_do_not_fit_refused(dev):
+    from mobilefinetuner_amd import gated_linear as L
+    x, W, g = torch.zeros(2, 8, device=dev), torch.zeros(8, 6, device=dev), torch.zeros(2, 6, device=dev)
+    for bad in (lambda: L.gated_linear(x, W, W[:, :5]), lambda: L.gated_linear(x, W, W.bfloat16()),
+                lambda: L.gated_linear(x, W.cpu(), W), lambda: L.gated_linear(x[:, :7], W, W),
+                lambda: L.gated_linear(x, W, W, "none"), lambda: L.gated_linear(x, W, W, w_transposed=True),
+                lambda: L.gated_linear(x, W[None], W[None]), lambda: L.gated_linear(x.half(), W.half(), W.half()),
+                lambda: L.gated_linear_backward(x, W, W, g, g, g[:1]), lambda: L.gated_linear_backward(x, W, W, None, g, g),
+                lambda: L.gated_linear_backward(x, W, W, g, g.bfloat16(), g)):
+        with pytest.raises(ValueError):
+            bad()
