@@ -233,7 +233,8 @@ mft_status mft_gated_linear_bwd(const mft_gated_linear_desc* desc, const void* x
 mft_status mft_gated_linear_e4m3_workspace_size(const mft_gated_linear_desc* desc, size_t* bytes) {
     const mft_status r = check(desc, "mft_gated_linear_e4m3_workspace_size", true);
     if (r != MFT_OK) return r;
-    if (bytes) *bytes = 0;
+    const mft::LinearProduct g = product_fwd(desc);
+    if (bytes) *bytes = desc->N == 0 || mft::few_rows(g) ? 0 : mft::gated_e4m3_workspace(g);
     return MFT_OK;
 }
 
@@ -243,8 +244,23 @@ mft_status mft_gated_linear_e4m3_fwd(const mft_gated_linear_desc* desc, const vo
     const char* who = "mft_gated_linear_e4m3_fwd";
     const mft_status r = check(desc, who, true);
     if (r != MFT_OK) return r;
-    (void)x_scale, (void)gate_scale, (void)up_scale, (void)x, (void)W_gate, (void)W_up, (void)h, (void)workspace, (void)stream;
-    return fail(MFT_ERR_UNSUPPORTED, "mft_gated_linear_e4m3_fwd: not built");
+    if (desc->N == 0) return MFT_OK;
+    if (!x || !x_scale || !W_gate || !gate_scale || !W_up || !up_scale || !h)
+        return fail(MFT_ERR_INVALID_ARG, "mft_gated_linear_e4m3_fwd: operands, scales and h must be non-NULL");
+    if (any_is(h, {x, x_scale, W_gate, gate_scale, W_up, up_scale}))
+        return fail(MFT_ERR_INVALID_ARG, "mft_gated_linear_e4m3_fwd: h may not be an operand");
+    mft::LinearProduct g = product_fwd(desc);
+    g.P = x;
+    g.Q = W_gate;
+    g.Q2 = W_up;
+    g.C = h;
+    g.partial = static_cast<float*>(workspace);
+    if (mft::few_rows(g))
+        return hip_status(mft::launch_gated_rows_e4m3(g, x_scale, gate_scale, up_scale, stream),
+                          "mft_gated_linear_e4m3_fwd launch");
+    if (!workspace && mft::gated_e4m3_workspace(g) > 0)
+        return fail(MFT_ERR_INVALID_ARG, "mft_gated_linear_e4m3_fwd: workspace must be non-NULL");
+    return hip_status(mft::launch_gated_e4m3(g, x_scale, gate_scale, up_scale, stream), "mft_gated_linear_e4m3_fwd launch");
 }
 
 }  // extern "C"

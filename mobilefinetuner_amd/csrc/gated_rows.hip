@@ -16,16 +16,42 @@
 
 #include "attn_geometry.h"
 #include "attn_kernels.h"
+#include "e4m3.h"
 #include "linear_epilogue.h"
 #include "row_util.h"
 
 namespace mft {
 namespace {
 
+// The storage of e4m3 numbers, and what their product needs beside the weights.
+struct e4m3 {
+    uint8_t bits;
+};
+struct Scales {
+    const float *x, *gate, *up;
+};
+
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
+template <typename T, int V> __device__ __forceinline__ void load_row(const T* row, int64_t k, int64_t K, float* x) {
+    load_part<T, V>(row, k, K, x);
+}
+template <> __device__ __forceinline__ void load_row<e4m3, 16>(const e4m3* row, int64_t k, int64_t K, float* x) {
+    typedef uint32_t word __attribute__((ext_vector_type(4)));
+    typedef word any16 __attribute__((aligned(1)));
+    word v{};
+    if (k + 16 <= K) {
+        v = *reinterpret_cast<const any16*>(row + k);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (k + e < K) v[e / 4] |= (uint32_t)row[k + e].bits << (8 * (e & 3));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e4m3_unpack4(v[i], x + 4 * i);
+}
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 
-template <typename T, int MR, int COLS> __global__ __launch_bounds__(256) void gated_rows_kc(LinearProduct g) {
+template <typename T, int MR, int COLS> __global__ __launch_bounds__(256) void gated_rows_kc(LinearProduct g, Scales s) {
     constexpr int V = kVec<T>, R = 2 * COLS;  // rows of the weights: gate's, then up's
     const int lane = threadIdx.x & 63;
     const int64_t n0 = ((int64_t)xcd_block((int)blockIdx.x, (int)gridDim.x) * 4 + wave_id()) * COLS;
@@ -36,9 +62,9 @@ template <typename T, int MR, int COLS> __global__ __launch_bounds__(256) void g
     for (int64_t k = (int64_t)lane * V; k < g.K; k += 64 * V) {
         float q[R][V], p[MR][V];
 #pragma unroll
-        for (int r = 0; r < R; ++r) load_part<T, V>(Q[r / COLS] + min(n0 + r % COLS, g.N - 1) * g.K, k, g.K, q[r]);
+        for (int r = 0; r < R; ++r) load_row<T, V>(Q[r / COLS] + min(n0 + r % COLS, g.N - 1) * g.K, k, g.K, q[r]);
 #pragma unroll
-        for (int m = 0; m < MR; ++m) load_part<T, V>(P + min<int64_t>(m, g.M - 1) * g.K, k, g.K, p[m]);
+        for (int m = 0; m < MR; ++m) load_row<T, V>(P + min<int64_t>(m, g.M - 1) * g.K, k, g.K, p[m]);
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -55,7 +81,14 @@ template <typename T, int MR, int COLS> __global__ __launch_bounds__(256) void g
             if (lane == c + COLS * m) gate = a, up = b;
         }
     const int64_t n = n0 + lane % COLS, m = lane / COLS;
-    if (m < min<int64_t>(MR, g.M) && n < g.N) gated_epilogue<T, 1>(g, m, n, &gate, &up);
+    if (m >= min<int64_t>(MR, g.M) || n >= g.N) return;
+    if constexpr (std::is_same_v<T, e4m3>) {
+        gate = gate * s.x[m] * s.gate[n];
+        up = up * s.x[m] * s.up[n];
+        gated_epilogue<bf16, 1>(g, m, n, &gate, &up);
+    } else {
+        gated_epilogue<T, 1>(g, m, n, &gate, &up);
+    }
 }
 
 // CH: lanes to a workgroup's columns (CH * V of them).
@@ -103,13 +136,13 @@ template <typename T, int MR, int CH> __global__ __launch_bounds__(kThreads) voi
     }
 }
 
+template <typename T, int MR> void launch_kc(const LinearProduct& g, const Scales& s, hipStream_t st) {
+    auto waves = [&](int cols) { return dim3((unsigned)((g.N + 4 * cols - 1) / (4 * cols))); };
+    if (g.N >= 16 * device_cus()) hipLaunchKernelGGL((gated_rows_kc<T, MR, 2>), waves(2), dim3(256), 0, st, g, s);
+    else hipLaunchKernelGGL((gated_rows_kc<T, MR, 1>), waves(1), dim3(256), 0, st, g, s);
+}
 template <typename T, int MR> void launch_m(const LinearProduct& g, hipStream_t st) {
-    if (g.q_kc) {
-        auto waves = [&](int cols) { return dim3((unsigned)((g.N + 4 * cols - 1) / (4 * cols))); };
-        if (g.N >= 16 * device_cus()) hipLaunchKernelGGL((gated_rows_kc<T, MR, 2>), waves(2), dim3(256), 0, st, g);
-        else hipLaunchKernelGGL((gated_rows_kc<T, MR, 1>), waves(1), dim3(256), 0, st, g);
-        return;
-    }
+    if (g.q_kc) return launch_kc<T, MR>(g, Scales{}, st);
     auto grid = [&](int ch) { return dim3((unsigned)((g.N + ch * kVec<T> - 1) / (ch * kVec<T>))); };
     const int64_t few = device_cus() / 2;
     if (g.N / (8 * kVec<T>) >= few) hipLaunchKernelGGL((gated_rows_nkc<T, MR, 8>), grid(8), dim3(kThreads), 0, st, g);
@@ -124,6 +157,15 @@ hipError_t launch_gated_rows(const LinearProduct& g, bool is_bf16, hipStream_t s
     if (!few_rows(g)) return hipErrorInvalidValue;
     if (is_bf16) g.M == 1 ? launch_m<bf16, 1>(g, st) : launch_m<bf16, 2>(g, st);
     else g.M == 1 ? launch_m<float, 1>(g, st) : launch_m<float, 2>(g, st);
+    return hipGetLastError();
+}
+
+hipError_t launch_gated_rows_e4m3(const LinearProduct& g, const float* x_scale, const float* gate_scale,
+                                  const float* up_scale, hipStream_t st) {
+    if (g.M <= 0 || g.N <= 0 || g.K <= 0) return hipSuccess;
+    if (!few_rows(g) || !g.q_kc) return hipErrorInvalidValue;
+    const Scales s{x_scale, gate_scale, up_scale};
+    g.M == 1 ? launch_kc<e4m3, 1>(g, s, st) : launch_kc<e4m3, 2>(g, s, st);
     return hipGetLastError();
 }
 

@@ -48,7 +48,14 @@ hipError_t launch_gated_gemm(const LinearProduct& g, hipStream_t st);
 // hold `joint` k each and K = 2 joint (gated_gemm.hip).
 size_t joined_gemm_workspace(const LinearProduct& g);
 hipError_t launch_joined_gemm(const LinearProduct& g, hipStream_t st);
-// Few rows (gated_rows.hip); no workspace.
+// The gated product of e4m3 numbers with a scale for each row of P, Q and Q2, all with k contiguous, C in
+// bf16 (gated_e4m3.hip).
+size_t gated_e4m3_workspace(const LinearProduct& g);
+hipError_t launch_gated_e4m3(const LinearProduct& g, const float* x_scale, const float* gate_scale,
+                             const float* up_scale, hipStream_t st);
+// The same and the gated product of either type for few rows (gated_rows.hip); no workspace.
+hipError_t launch_gated_rows_e4m3(const LinearProduct& g, const float* x_scale, const float* gate_scale,
+                                  const float* up_scale, hipStream_t st);
 hipError_t launch_gated_rows(const LinearProduct& g, bool bf16, hipStream_t st);
 // dz[N, 2 ld] = (dh up act'(gate) | dh act(gate)), either half padded with zeros from ff to ld columns
 // (gated.hip).
