@@ -189,6 +189,13 @@ __device__ __forceinline__ void write_rows(const Args& a, int slice, int64_t mw,
             *reinterpret_cast<f32x4*>(st + (lane & 31) * kPitch + 32 * j + 8 * q + 4 * (lane >> 5)) =
                 f32x4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
     asm volatile("" ::: "memory");  // a wave's LDS accesses stay in order
+    if constexpr (MODE == GATED) {
+        if (a.whole) {
+            gated_rows_out<COLS, kPitch, false>(a.g, mw, nw, st, lane, nullptr, nullptr, nullptr);
+            asm volatile("" ::: "memory");
+            return;
+        }
+    }
 #pragma unroll
     for (int r = 0; r < LPR / 2; ++r) {
         const int at = r * 64 + lane, row = at / LPR, c = at % LPR * V;
@@ -202,14 +209,12 @@ __device__ __forceinline__ void write_rows(const Args& a, int slice, int64_t mw,
                 const f32x4 u = *reinterpret_cast<const f32x4*>(st + row * kPitch + i * COLS + c + e);
                 v[i][e] = u[0], v[i][e + 1] = u[1], v[i][e + 2] = u[2], v[i][e + 3] = u[3];
             }
-        if (!a.whole) {
+        if (MODE != GATED && a.whole) {
+            linear_epilogue<bf16, ACT, V>(a.g, m, n, v[0]);
+        } else {
 #pragma unroll
             for (int i = 0; i < NQ; ++i)
                 store_part<float, V>(a.g.partial + (((int64_t)slice * NQ + i) * a.g.M + m) * a.g.N, n, a.g.N, v[i]);
-        } else if constexpr (MODE == GATED) {
-            gated_epilogue<bf16, V>(a.g, m, n, v[0], v[1]);
-        } else {
-            linear_epilogue<bf16, ACT, V>(a.g, m, n, v[0]);
         }
     }
     asm volatile("" ::: "memory");

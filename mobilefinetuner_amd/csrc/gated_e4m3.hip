@@ -6,13 +6,13 @@
 // sums of a column in one lane, on v_mfma_f32_32x32x64_f8f6f4 (without block scales:
 // a row's scale leaves the sum).  It multiplies 64 k in the time of 32 in bf16, so in
 // bytes loads, LDS and matrix units are in the ratio of bf_gemm_tiles.h, whose slabs
-// these are: [rows][128 bytes], direct loads, RING of them in LDS.  The 32 bytes of a
+// these are: [rows][128 bytes], direct loads, two of them in LDS.  The 32 bytes of a
 // lane's fragment are two 16-byte reads; which k they hold is the same for all
 // operands.
 //
 // A pair of halves of 64 k to a slab: while a half is multiplied the next one's
 // fragments are read.  Behind the barrier after a slab's last reads the loads of the
-// slab RING further on go out into it.
+// slab after the next go out into it.
 //
 // What the matrix unit keeps.  It adds the products of eight consecutive k first, each
 // cut towards zero to a multiple of 2^-13 of 2^(a + b), a and b the exponents of the
@@ -80,7 +80,7 @@ template <int R> struct Rows {
 template <int TN>
 __device__ __forceinline__ void write_h(const E4m3Args& a, int64_t mw, int64_t nw, const f32x16 (&acc)[TN], float* st,
                                         int lane) {
-    constexpr int COLS = 16 * TN, V = 8, LPR = COLS / V, kPitch = 2 * COLS + 4;
+    constexpr int COLS = 16 * TN, kPitch = 2 * COLS + 4;
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -88,33 +88,13 @@ __device__ __forceinline__ void write_h(const E4m3Args& a, int64_t mw, int64_t n
             *reinterpret_cast<f32x4*>(st + (lane & 31) * kPitch + 32 * j + 8 * q + 4 * (lane >> 5)) =
                 f32x4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
     asm volatile("" ::: "memory");  // a wave's LDS accesses stay in order
-    const LinearProduct& g = a.a.g;
-    const int64_t n = nw + lane % LPR * V;
-    float gs[V], us[V];
-    load_part<float, V>(a.gate_scale, n, g.N, gs);
-    load_part<float, V>(a.up_scale, n, g.N, us);
-#pragma unroll
-    for (int r = 0; r < LPR / 2; ++r) {
-        const int row = (r * 64 + lane) / LPR, c = lane % LPR * V;
-        const int64_t m = mw + row;
-        if (m >= g.M || n >= g.N) continue;
-        const float xs = a.x_scale[m];
-        float v[2][V];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < V; e += 4) {
-                const f32x4 u = *reinterpret_cast<const f32x4*>(st + row * kPitch + i * COLS + c + e);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) v[i][e + x] = u[x] * xs * (i ? us : gs)[e + x];
-            }
-        gated_epilogue<bf16, V>(g, m, n, v[0], v[1]);
-    }
+    gated_rows_out<COLS, kPitch, true>(a.a.g, mw, nw, st, lane, a.x_scale, a.gate_scale, a.up_scale);
     asm volatile("" ::: "memory");
 }
 
-template <int BN, int BM, int RING>
-__global__ __launch_bounds__(kThreads, BN * BM > 32768 || RING > 2 ? 1 : 2) void gated_e4m3_kernel(E4m3Args a) {
+template <int BN, int BM>
+__global__ __launch_bounds__(kThreads, BN * BM > 32768 ? 1 : 2) void gated_e4m3_kernel(E4m3Args a) {
+    constexpr int RING = 2;
     constexpr int TN = BN / 64, TM = BM / 64, TQ = TN / 2, kTiles = TN * TM, kFrags = TN + TM;
     typedef Rows<BM> OpP;
     typedef Rows<BN / 2> OpQ;
@@ -255,11 +235,37 @@ __global__ __launch_bounds__(kThreads, BN * BM > 32768 || RING > 2 ? 1 : 2) void
     }
 }
 
-template <int BN, int BM, int RING> hipError_t launch_t(E4m3Args a, hipStream_t st) {
+// The tiles (columns of both sums together), the workgroups that a CU holds, and
+// what one takes in us: with one to a CU at, and with more, a + b K.  Fitted to 41
+// sizes of 16 to 8192 rows and 640 to 8192 columns.  8192 x 1152 -> 6912 151 us in 128 x
+// 192, 169 in 128 x 128, 182 in 256 x 256, whose epilogue nothing hides; 4096 x 4096
+// -> 8192 254, 294 and 236: over long k it reads LDS least.  256 rows of it 25 us in 128 x
+// 64, 28 in 128 x 128, 45 in 256 x 256.
+struct Shape {
+    int bn, bm, at_once;
+    double one_a, one_b, a, b;
+};
+constexpr Shape kShapes[] = {{256, 256, 1, 14, 0.0109, 14, 0.0109}, {128, 192, 2, 7.5, 0.0080, 7.5, 0.0091},
+                             {128, 128, 2, 6, 0.0054, 4.4, 0.0079}, {128, 64, 3, 5.4, 0.0047, 2.5, 0.0071}};
+int shape_of(const LinearProduct& g) {
+    const double cus = device_cus();
+    int best = 0;
+    double least = 1e300;
+    for (int i = 0; i < 4; ++i) {
+        const Shape& t = kShapes[i];
+        const double tiles = (double)((2 * g.N + t.bn - 1) / t.bn) * ((g.M + t.bm - 1) / t.bm);
+        const double rounds = std::max(1.0, tiles / (cus * t.at_once));
+        const double us = tiles <= cus ? t.one_a + t.one_b * g.K : (std::ceil(rounds) + rounds) / 2 * (t.a + t.b * g.K);
+        if (us < least) least = us, best = i;
+    }
+    return best;
+}
+
+template <int BN, int BM> hipError_t launch_t(E4m3Args a, hipStream_t st) {
     a.a.tiles_m = (int)((a.a.g.M + BM - 1) / BM);
     a.a.tiles_n = (int)((2 * a.a.g.N + BN - 1) / BN);
     a.a.per_slice_tiles = FastDiv::make((uint32_t)(a.a.tiles_m * a.a.tiles_n));
-    hipLaunchKernelGGL((gated_e4m3_kernel<BN, BM, RING>), dim3((unsigned)(a.a.tiles_m * a.a.tiles_n)), dim3(kThreads), 0,
+    hipLaunchKernelGGL((gated_e4m3_kernel<BN, BM>), dim3((unsigned)(a.a.tiles_m * a.a.tiles_n)), dim3(kThreads), 0,
                        st, a);
     return hipGetLastError();
 }
@@ -311,12 +317,12 @@ hipError_t launch_gated_e4m3(const LinearProduct& given, const float* x_scale, c
     a.a.g = g;
     a.x_scale = x_scale, a.gate_scale = gate_scale, a.up_scale = up_scale;
     a.slabs = on16(g.P) && on16(g.Q) && on16(g.Q2) && g.K <= (1 << 23) ? (int)(g.K / kRow) : 0;
-    const int64_t cus = device_cus();
-    auto tiles = [&](int64_t bn, int64_t bm) { return ((2 * g.N + bn - 1) / bn) * ((g.M + bm - 1) / bm); };
-    if (tiles(256, 256) >= 2 * cus) return launch_t<256, 256, 2>(a, st);
-    if (tiles(256, 128) >= cus) return launch_t<256, 128, 3>(a, st);
-    if (tiles(128, 128) >= cus) return launch_t<128, 128, 2>(a, st);
-    return launch_t<128, 64, 2>(a, st);
+    switch (shape_of(g)) {
+        case 0: return launch_t<256, 256>(a, st);
+        case 1: return launch_t<128, 192>(a, st);
+        case 2: return launch_t<128, 128>(a, st);
+        default: return launch_t<128, 64>(a, st);
+    }
 }
 
 }  // namespace mft

@@ -45,17 +45,34 @@ struct Plan {
 };
 
 // The tiles (columns of both sums together), and what each sustains over the whole
-// GPU (TFLOP/s) with one workgroup to a CU and with more, and the k that its
-// prologue and epilogue are worth.
+// GPU (TFLOP/s) with one workgroup to a CU and with more, and the k that its prologue
+// and epilogue are worth (`act` of a gated tile: three outputs and the activation).
+// Fitted to five (GATED) and four (JOINED) pairs of widths from 640 to 8192 and 16
+// to 8192 rows, each timed in every tile and cut into 1 to 12 slices: the choice by
+// these is within 6 percent of the fastest in 74 of 86 (10 in 82; 1.29 times it in one)
+// and in 60 of 64 (10 in 63).
+//   256 x 256, one wave to a SIMD: 8192 x 1152 -> 6912, both sums kept, 267 us, W [in,
+//     ff] 268; 256 x 128 275, 128 x 128 320, the deep 256 x 128 340.  Its products
+//     alone are 183 (1430 TFLOP/s, what the card's power allows); the rest is a
+//     tile's beginning and its epilogue, which nothing hides.  Tiles of 128 x 192, two
+//     workgroups to a CU, hide it but read LDS more: 280, and 92 for 97 without the sums
+//     kept at K 640.
+//   deep, and 128 x 64: few tiles.  512 rows of it 25 us in the deep 256 x 128, 33 in
+//     256 x 256; 64 rows 13 us in the deep 128 x 128, 26.
 struct Shape {
     int bn, bm, deep;
     double one, more;
     int k, act;
 };
-constexpr Shape kShapes[] = {{256, 128, 0, 1000, 1350, 330, 190}, {128, 128, 0, 900, 1080, 345, 190},
-                             {128, 64, 0, 600, 900, 250, 100},    {256, 256, 0, 1400, 1540, 704, 200},
-                             {128, 128, 1, 1200, 1200, 380, 190}, {256, 128, 1, 1520, 1200, 380, 190}};
-constexpr int kShapeCount = sizeof(kShapes) / sizeof(kShapes[0]);
+constexpr int kShapeCount = 6;
+constexpr Shape kGated[kShapeCount] = {{256, 128, 0, 880, 1360, 200, 270}, {128, 128, 0, 970, 1120, 220, 250},
+                                       {128, 64, 0, 580, 780, 180, 80},    {256, 256, 0, 1460, 1480, 370, 200},
+                                       {128, 128, 1, 1330, 1010, 350, 80}, {256, 128, 1, 1440, 1520, 580, 420}};
+constexpr Shape kJoined[kShapeCount] = {{256, 128, 0, 890, 1180, 140, 0}, {128, 128, 0, 880, 1000, 490, 0},
+                                        {128, 64, 0, 490, 780, 170, 0},   {256, 256, 0, 1520, 1400, 430, 0},
+                                        {128, 128, 1, 1210, 1000, 390, 0}, {256, 128, 1, 1250, 1520, 710, 0}};
+// A second launch, and the partials written and read (bytes a us).
+constexpr double kKcGated = 1.07, kKcJoined = 1.15, kCutGated = 3.9, kCutJoined = 1.0, kCutRate = 4.3e6, kCutRateJoined = 3e6;
 // With k contiguous in both operands the slabs of 256 x 128 do not leave a CU room
 // for two; 64 rows of a deep slab are not whole rows of its eight waves' loads without.
 bool has_shape(const LinearProduct& g, int s, bool gated) {
@@ -69,20 +86,20 @@ Plan plan(const LinearProduct& g, bool gated) {
     int per = 1;
     for (int s = 0; s < kShapeCount; ++s) {
         if (!has_shape(g, s, gated)) continue;
-        const Shape& t = kShapes[s];
+        const Shape& t = (gated ? kGated : kJoined)[s];
         const int64_t tiles = ((g.N * nq + t.bn - 1) / t.bn) * ((g.M + t.bm - 1) / t.bm);
         for (int slices : {1, 2, 3, 4, 6, 8, 12, 16}) {
             if (slices > 1 && (slices > pairs || tiles * slices > 4 * cus)) break;
             const int per_slice = std::max(1, (pairs + slices - 1) / slices), n = std::max(1, (pairs + per_slice - 1) / per_slice);
             const double mean = (double)tiles * n / cus, most = std::ceil(mean);
-            const double rate = (most <= 1 ? t.one : t.more) * (g.q_kc ? 1.08 : 1.0) * cus / 256;
+            const double rate = (most <= 1 ? t.one : t.more) * (g.q_kc ? (gated ? kKcGated : kKcJoined) : 1.0) * cus / 256;
             double us = (most <= 1 ? 1 : t.deep ? most : (most + mean) / 2) * cus * t.bn * t.bm * 2 *
-                        ((double)g.K / n + t.k + (gated && n == 1 ? t.act : 0)) / rate / 1e6;
-            if (n > 1) us += 1 + (double)n * g.M * g.N * nq * 8 / 5.4e6;  // partials written and read, a launch
+                        ((double)g.K / n + t.k + (n == 1 ? t.act : 0)) / rate / 1e6;
+            if (n > 1) us += (gated ? kCutGated : kCutJoined) + (double)n * g.M * g.N * nq * 8 / (gated ? kCutRate : kCutRateJoined);
             if (us < best * 0.999) best = us, p.shape = s, per = per_slice;
         }
     }
-    const Shape& t = kShapes[p.shape];
+    const Shape& t = (gated ? kGated : kJoined)[p.shape];
     p.a.g = g;
     p.a.tiles_m = (int)((g.M + t.bm - 1) / t.bm);
     p.a.tiles_n = (int)((g.N * nq + t.bn - 1) / t.bn);

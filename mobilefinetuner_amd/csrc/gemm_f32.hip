@@ -192,8 +192,9 @@ template <int VEC> __device__ __forceinline__ void run_epilogue(const GemmF32& g
         float gate[VEC];
         if (g.z) store_part<float, VEC>(g.z + m * g.N, n, g.N, v);
         load_part<float, VEC>(g.gate + m * g.N, n, g.N, gate);
+        const Act act = Act::of(g.act);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] *= act_value_of(g.act, gate[e]);
+        for (int e = 0; e < VEC; ++e) v[e] *= act.value(gate[e]);
         store_part<float, VEC>(g.C + m * g.N, n, g.N, v);
         return;
     }

@@ -40,12 +40,21 @@ template <int ACT> __device__ __forceinline__ float act_grad(float z) {
     return 1.f;
 }
 
-// The same by an activation that a launch's threads share.
-__device__ __forceinline__ float act_value_of(int act, float z) {
-    return act == ACT_GELU_TANH ? act_value<ACT_GELU_TANH>(z) : act == ACT_SILU ? act_value<ACT_SILU>(z) : act_value<ACT_RELU>(z);
-}
-__device__ __forceinline__ float act_grad_of(int act, float z) {
-    return act == ACT_GELU_TANH ? act_grad<ACT_GELU_TANH>(z) : act == ACT_SILU ? act_grad<ACT_SILU>(z) : act_grad<ACT_RELU>(z);
-}
+// An activation that a launch's threads share, without a branch: GELU and SiLU are
+// z / (1 + exp2(z (c1 + c3 z^2))), and ReLU is chosen by a uniform condition.
+struct Act {
+    float c1, c3;
+    bool relu;
+    static __host__ __device__ Act of(int act) {
+        if (act == ACT_GELU_TANH) return {-2.f * kLog2e * kGeluC, -2.f * kLog2e * kGeluC * kGeluA, false};
+        return {-kLog2e, 0.f, act == ACT_RELU};
+    }
+    __device__ __forceinline__ float smooth(float z) const {
+        // below infinity, which c3 of 0 would make NaN; a NaN stays by z
+        const float x = z * fmaf(fminf(z * z, 3e38f), c3, c1);
+        return z * __builtin_amdgcn_rcpf(1.f + fast_exp2(x));
+    }
+    __device__ __forceinline__ float value(float z) const { return relu ? (z <= 0.f ? 0.f : z) : smooth(z); }
+};
 
 }  // namespace mft

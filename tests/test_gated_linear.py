@@ -187,11 +187,13 @@ def check_e4m3(dev, N, n_in, n_ff, act, seed, shift=0, near=False):
     within(h, rh, th, "h")
 
 
-# the shapes above, and every tile: of 256 x 256, 256 x 128, 128 x 128 and 128 x 64, whole and ragged
+# the shapes above, and every tile: of 256 x 256, 128 x 192, 128 x 128 and 128 x 64, whole and ragged
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", SHAPES + [(3, 128, 64), (65, 144, 100), (2048, 256, 8192), (2100, 272, 8200),
                                             (512, 640, 8192), (500, 208, 8190), (256, 128, 8192), (250, 272, 8100),
-                                            (33, 4096, 128), (2000, 601, 1999)],
+                                            (33, 4096, 128), (2000, 601, 1999), (1024, 4096, 8192),
+                                            (1000, 4112, 8200), (8192, 1152, 2048), (8190, 1168, 2046),
+                                            (2048, 2048, 1024), (2000, 2064, 1000)],
                          ids=lambda s: "x".join(map(str, s)))
 def test_eight_bits(dev, shape):
     check_e4m3(dev, *shape, "gelu_tanh", sum(shape))
