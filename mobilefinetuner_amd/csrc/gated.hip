@@ -1,5 +1,6 @@
-// The element-wise pass of the gated linear layer's backward (C ABI in
-// include/mft/gated_linear.h): the gradients of both sums.  Bound by memory.
+// The element-wise passes of the gated linear layer's backward (C ABI in
+// include/mft/gated_linear.h): the gradients of both sums, and small weights laid
+// beside one another.  Bound by memory.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -57,7 +58,28 @@ void dz_t(const void* gate, const void* up, const void* dh, void* dz, int64_t N,
 #undef MFT_GATED_DZ
 }
 
+// Two weights [rows, cols] beside one another, [rows, 2 cols], or one below the other.
+__global__ __launch_bounds__(256) void join_weights(const float* a, const float* b, float* to, int64_t rows, int64_t cols,
+                                                    int beside) {
+    const int64_t chunks = (cols + 3) / 4, n = rows * chunks, step = (int64_t)gridDim.x * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += step) {
+        const int64_t j = i < n ? i : i - n, r = j / chunks, c = (j - r * chunks) * 4;
+        float v[4];
+        load_part<float, 4>((i < n ? a : b) + r * cols, c, cols, v);
+        float* row = beside ? to + (2 * r + (i >= n)) * cols : to + (r + (i < n ? 0 : rows)) * cols;
+        store_part<float, 4>(row, c, cols, v);
+    }
+}
+
 }  // namespace
+
+hipError_t launch_join_weights(const float* a, const float* b, float* to, int64_t rows, int64_t cols, bool beside,
+                               hipStream_t st) {
+    const int64_t n = 2 * rows * ((cols + 3) / 4);
+    hipLaunchKernelGGL(join_weights, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 16 * device_cus())), dim3(256), 0, st,
+                       a, b, to, rows, cols, (int)beside);
+    return hipGetLastError();
+}
 
 hipError_t launch_gated_dz(const void* gate, const void* up, const void* dh, void* dz, int64_t N, int64_t ff, int64_t ld,
                            int act, bool is_bf16, hipStream_t st) {

@@ -6,8 +6,9 @@
 // by the M rows' in fp32 in the lane that has loaded it, 16 bytes a lane; sums meet
 // in registers and, across waves, in LDS, in an order that the sizes fix.
 //
-// With k contiguous a wave takes two rows of either weight, or one where that
-// leaves fewer than eight waves to a CU, and its lanes share k.  With its rows
+// With k contiguous a wave takes one row of either weight, or two from 32 waves to a
+// CU on, and its lanes share k.  bf16, one row, weights out of cache: 896 -> 4864 6.8 us
+// (two rows 7.1), 1152 -> 6912 10.6 (10.2; 3.1 TB/s), 4096 -> 8192 25.9 (24.9; 5.4 TB/s).  With its rows
 // contiguous a workgroup takes 64 consecutive n or fewer of both (so that about 128
 // workgroups run) and its lanes' groups share k.
 #include <hip/hip_runtime.h>
@@ -32,24 +33,37 @@ struct Scales {
 };
 
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
-template <typename T, int V> __device__ __forceinline__ void load_row(const T* row, int64_t k, int64_t K, float* x) {
-    load_part<T, V>(row, k, K, x);
-}
-template <> __device__ __forceinline__ void load_row<e4m3, 16>(const e4m3* row, int64_t k, int64_t K, float* x) {
-    typedef uint32_t word __attribute__((ext_vector_type(4)));
-    typedef word any16 __attribute__((aligned(1)));
-    word v{};
-    if (k + 16 <= K) {
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// 16 bytes of a row of K from element k on, zeros past its end.
+template <typename T> __device__ __forceinline__ u32x4 load16(const T* row, int64_t k, int64_t K) {
+    typedef u32x4 any16 __attribute__((aligned(1)));
+    constexpr int V = kVec<T>;
+    u32x4 v{};
+    if (k + V <= K) {
         v = *reinterpret_cast<const any16*>(row + k);
+    } else if (k < K) {
+        T part[V] = {};
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (k + e < K) part[e] = row[k + e];
+        v = __builtin_bit_cast(u32x4, part);
+    }
+    return v;
+}
+template <typename T> __device__ __forceinline__ void unpack(u32x4 v, float* x) {
+    if constexpr (std::is_same_v<T, e4m3>) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e4m3_unpack4(v[i], x + 4 * i);
+    } else if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v[i]);
     } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-            if (k + e < K) v[e / 4] |= (uint32_t)row[k + e].bits << (8 * (e & 3));
+        for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(v[i] << 16), x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) e4m3_unpack4(v[i], x + 4 * i);
 }
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kAhead = 4;
 
 template <typename T, int MR, int COLS> __global__ __launch_bounds__(256) void gated_rows_kc(LinearProduct g, Scales s) {
     constexpr int V = kVec<T>, R = 2 * COLS;  // rows of the weights: gate's, then up's
@@ -58,19 +72,33 @@ template <typename T, int MR, int COLS> __global__ __launch_bounds__(256) void g
     if (n0 >= g.N) return;
     const T *P = (const T*)g.P, *Q[2] = {(const T*)g.Q, (const T*)g.Q2};
     float acc[R][MR] = {};
-#pragma unroll 4
-    for (int64_t k = (int64_t)lane * V; k < g.K; k += 64 * V) {
-        float q[R][V], p[MR][V];
+    // All loads of kAhead rounds go out before the first is used, whatever K is: one round at a time a row of
+    // 1152 was three round trips, 13.5 us for 1 x 1152 -> 6912 in bf16.
+    for (int64_t k0 = (int64_t)lane * V; k0 < g.K; k0 += kAhead * 64 * V) {
+        u32x4 q[kAhead][R], p[kAhead][MR];
 #pragma unroll
-        for (int r = 0; r < R; ++r) load_row<T, V>(Q[r / COLS] + min(n0 + r % COLS, g.N - 1) * g.K, k, g.K, q[r]);
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t k = k0 + u * 64 * V;
 #pragma unroll
-        for (int m = 0; m < MR; ++m) load_row<T, V>(P + min<int64_t>(m, g.M - 1) * g.K, k, g.K, p[m]);
+            for (int r = 0; r < R; ++r) q[u][r] = load16(Q[r / COLS] + min(n0 + r % COLS, g.N - 1) * g.K, k, g.K);
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+            for (int m = 0; m < MR; ++m) p[u][m] = load16(P + min<int64_t>(m, g.M - 1) * g.K, k, g.K);
+        }
 #pragma unroll
-            for (int m = 0; m < MR; ++m)
+        for (int u = 0; u < kAhead; ++u) {
+            float x[MR][V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) acc[r][m] = fmaf(q[r][e], p[m][e], acc[r][m]);
+            for (int m = 0; m < MR; ++m) unpack<T>(p[u][m], x[m]);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float w[V];
+                unpack<T>(q[u][r], w);
+#pragma unroll
+                for (int m = 0; m < MR; ++m)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) acc[r][m] = fmaf(w[e], x[m][e], acc[r][m]);
+            }
+        }
     }
     float gate = 0.f, up = 0.f;  // lane c + COLS m has column c of row m
 #pragma unroll
@@ -138,7 +166,7 @@ template <typename T, int MR, int CH> __global__ __launch_bounds__(kThreads) voi
 
 template <typename T, int MR> void launch_kc(const LinearProduct& g, const Scales& s, hipStream_t st) {
     auto waves = [&](int cols) { return dim3((unsigned)((g.N + 4 * cols - 1) / (4 * cols))); };
-    if (g.N >= 16 * device_cus()) hipLaunchKernelGGL((gated_rows_kc<T, MR, 2>), waves(2), dim3(256), 0, st, g, s);
+    if (g.N >= 32 * device_cus()) hipLaunchKernelGGL((gated_rows_kc<T, MR, 2>), waves(2), dim3(256), 0, st, g, s);
     else hipLaunchKernelGGL((gated_rows_kc<T, MR, 1>), waves(1), dim3(256), 0, st, g, s);
 }
 template <typename T, int MR> void launch_m(const LinearProduct& g, hipStream_t st) {

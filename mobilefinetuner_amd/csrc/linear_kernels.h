@@ -57,6 +57,9 @@ hipError_t launch_gated_e4m3(const LinearProduct& g, const float* x_scale, const
 hipError_t launch_gated_rows_e4m3(const LinearProduct& g, const float* x_scale, const float* gate_scale,
                                   const float* up_scale, hipStream_t st);
 hipError_t launch_gated_rows(const LinearProduct& g, bool bf16, hipStream_t st);
+// Two fp32 weights [rows, cols] beside one another, [rows, 2 cols], or one below the other (gated.hip).
+hipError_t launch_join_weights(const float* a, const float* b, float* to, int64_t rows, int64_t cols, bool beside,
+                               hipStream_t st);
 // dz[N, 2 ld] = (dh up act'(gate) | dh act(gate)), either half padded with zeros from ff to ld columns
 // (gated.hip).
 hipError_t launch_gated_dz(const void* gate, const void* up, const void* dh, void* dz, int64_t N, int64_t ff, int64_t ld,

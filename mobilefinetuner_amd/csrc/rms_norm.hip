@@ -205,39 +205,46 @@ template <typename T, bool E4M3> __global__ __launch_bounds__(kLongThreads) void
 template <int WPR> constexpr int kBwdThreads = WPR == 1 ? 512 : 64 * WPR;
 
 // Workgroup g: rows in steps of groups * (rows a workgroup holds at once).  EVEN:
-// D is a multiple of the vector, so that no element is looked at by itself.
+// D is a multiple of the vector, so that no element is looked at by itself.  A row
+// stays in T between its two passes, over the sum and to dx: 16384 x 1152 in bf16 with
+// the stream's gradient 36 us (4.2 TB/s); in fp32 its registers leave eight waves to a
+// CU, 56 us.
 template <typename T, int WPR, int CH, bool PARAMS, bool EVEN>
-__global__ __launch_bounds__(kBwdThreads<WPR>) void rms_bwd(RmsNormArgs a) {
+__global__ __launch_bounds__(kBwdThreads<WPR>, WPR == 4 ? 2 : 4) void rms_bwd(RmsNormArgs a) {
     constexpr int V = kVec<T>, TPR = 64 * WPR, NT = kBwdThreads<WPR>, RPB = NT / TPR;
+    typedef typename AnyVec<T, V>::raw raw;
     __shared__ __attribute__((aligned(16))) float lds[PARAMS && RPB > 1 ? RPB / 2 * CH * V * 64 : 1];
     __shared__ float s[2][WPR];
     const int t = threadIdx.x % TPR;
     const float inv = 1.0f / (float)a.D;
     // Elements from d0 on, 0 past the row's end (and with it all below).
-    auto load = [&](auto* row, int64_t d0, float* x) {
-        typedef std::remove_const_t<std::remove_pointer_t<decltype(row)>> E;
-        if constexpr (EVEN) {
+    auto load = [&](const T* row, int64_t d0) {
+        raw x{};
+        if (d0 + (EVEN ? 0 : V - 1) < a.D) {
+            x = AnyVec<T, V>::load_raw(row + d0);
+        } else if (!EVEN) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[e] = 0.f;
-            if (d0 < a.D) AnyVec<E, V>::load(row + d0, x);
-        } else {
-            load_part<E, V>(row, d0, a.D, x);
+            for (int e = 0; e < V; ++e)
+                if (d0 + e < a.D) x[e] = row[d0 + e];
         }
+        return x;
     };
     float dw[CH][V], f[CH][V];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        if (a.w) load(a.w, (int64_t)(c * TPR + t) * V, f[c]);
+        factors<V>(a, (int64_t)(c * TPR + t) * V, f[c]);
 #pragma unroll
-        for (int e = 0; e < V; ++e) dw[c][e] = 0.f, f[c][e] = a.w ? f[c][e] + a.one : 1.f;
+        for (int e = 0; e < V; ++e) dw[c][e] = 0.f;
     }
     int turn = 0;
     for (int64_t n = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; n < a.N; n += a.groups * RPB) {
-        float h[CH][V], g[CH][V];
+        raw x[CH], g[CH], d[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            load((const T*)a.x + n * a.sx, (int64_t)(c * TPR + t) * V, h[c]);
-            load((const T*)a.dy + n * a.sdy, (int64_t)(c * TPR + t) * V, g[c]);
+            const int64_t d0 = (int64_t)(c * TPR + t) * V;
+            x[c] = load((const T*)a.x + n * a.sx, d0);
+            g[c] = load((const T*)a.dy + n * a.sdy, d0);
+            d[c] = a.dt ? load((const T*)a.dt + n * a.sdt, d0) : raw{};
         }
         const float rstd = a.rstd_in[n];
         float c2 = 0.f;
@@ -245,16 +252,11 @@ __global__ __launch_bounds__(kBwdThreads<WPR>) void rms_bwd(RmsNormArgs a) {
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                h[c][e] *= rstd;
-                if constexpr (PARAMS) dw[c][e] = fmaf(g[c][e], h[c][e], dw[c][e]);
-                g[c][e] *= f[c][e];
-                c2 = fmaf(g[c][e], h[c][e], c2);
+                const float h = (float)x[c][e] * rstd, gh = (float)g[c][e] * h;
+                if constexpr (PARAMS) dw[c][e] += gh;
+                c2 = fmaf(gh, f[c][e], c2);
             }
         if (a.dx) {
-            float d[CH][V];
-            if (a.dt)
-#pragma unroll
-                for (int c = 0; c < CH; ++c) load((const T*)a.dt + n * a.sdt, (int64_t)(c * TPR + t) * V, d[c]);
             c2 = row_sum<WPR>(c2, s[turn]) * inv;
             turn ^= 1;
             T* dr = (T*)a.dx + n * a.sdx;
@@ -262,13 +264,15 @@ __global__ __launch_bounds__(kBwdThreads<WPR>) void rms_bwd(RmsNormArgs a) {
             for (int c = 0; c < CH; ++c) {
                 const int64_t d0 = (int64_t)(c * TPR + t) * V;
                 if (d0 >= a.D) break;
+                asm volatile("" : "+v"(x[c]), "+v"(g[c]));  // T's registers, not fp32's, from the first pass on
+                float o[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    g[c][e] = rstd * (g[c][e] - h[c][e] * c2);
-                    if (a.dt) g[c][e] += d[c][e];
+                    o[e] = rstd * ((float)g[c][e] * f[c][e] - (float)x[c][e] * rstd * c2);
+                    if (a.dt) o[e] += (float)d[c][e];
                 }
-                if constexpr (EVEN) AnyVec<T, V>::store(dr + d0, g[c]);
-                else store_part<T, V>(dr, d0, a.D, g[c]);
+                if constexpr (EVEN) AnyVec<T, V>::store(dr + d0, o);
+                else store_part<T, V>(dr, d0, a.D, o);
             }
         }
     }
@@ -380,16 +384,18 @@ Shape fwd_shape(int64_t D, int vec) {
     return {0, 0};
 }
 Shape bwd_shape(int64_t D, int vec) {
-    for (const Shape s : {Shape{1, 1}, {1, 2}, {1, 3}, {4, 1}, {4, 2}, {4, 4}, {16, 2}})
+    for (const Shape s : {Shape{1, 1}, {1, 2}, {1, 3}, {4, 2}, {16, 1}, {16, 2}})
         if (D <= (int64_t)64 * s.wpr * s.ch * vec) return s;
     return {0, 0};
 }
+// Workgroups of the backward, each of which leaves a partial.  One to a CU, or two of
+// four waves from eight rows a CU on: 4096 x 1152 in fp32 18 us (one: 22), 1001 x 1153 12
+// (11); of eight waves a row each, 16384 x 1152 in bf16 36 (two: 38, four: 39), of
+// sixteen, 2048 x 8192 33 (two: 37).
 int64_t bwd_groups(int64_t N, int64_t D, int vec) {
     const Shape s = bwd_shape(D, vec);
-    const int64_t at_once = s.wpr == 1 ? 8 : 1, most = s.wpr == 16 || s.wpr == 0 ? 1 : s.wpr == 4 ? 4 : 2;
-    // few rows, a wave to each: one workgroup to a CU, as each leaves a partial
-    return std::max<int64_t>(1, std::min<int64_t>((N + at_once - 1) / at_once,
-                                                  (s.wpr == 1 && N < 64 * device_cus() ? 1 : most) * device_cus()));
+    const int64_t at_once = s.wpr == 1 ? 8 : 1, cus = device_cus();
+    return std::max<int64_t>(1, std::min<int64_t>((N + at_once - 1) / at_once, (s.wpr == 4 && N >= 8 * cus ? 2 : 1) * cus));
 }
 size_t up(size_t x) { return (x + 255) & ~size_t(255); }
 
@@ -467,9 +473,8 @@ template <typename T> hipError_t bwd(const RmsNormArgs& a, hipStream_t st) {
     MFT_RMS_BWD(1, 1)
     MFT_RMS_BWD(1, 2)
     MFT_RMS_BWD(1, 3)
-    MFT_RMS_BWD(4, 1)
     MFT_RMS_BWD(4, 2)
-    MFT_RMS_BWD(4, 4)
+    MFT_RMS_BWD(16, 1)
     MFT_RMS_BWD(16, 2)
 #undef MFT_RMS_BWD_E
 #undef MFT_RMS_BWD
