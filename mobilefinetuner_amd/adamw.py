@@ -4,7 +4,7 @@ weights and whole matrices.
 
 Parameters are fp32, or bf16 with an fp32 master copy among the states.  States
 are fp32 or 8 bits wide.  One step is two launches and one more for each further
-48 to 64 tensors (with clipping as many again, less one).  There is no CPU path.
+48 (8 bits) or 64 tensors, and with clipping one for each 120.  There is no CPU path.
 """
 from __future__ import annotations
 
@@ -20,7 +20,8 @@ from .device import guard, operand, ptr, stream, workspace
 GROUP = capi.ADAMW_GROUP  # values of an 8-bit state with one scale
 _FIELDS = C.sizeof(capi.AdamWTensor) // 8
 _GRAD = capi.AdamWTensor.grad.offset // 8
-_ADDRESS, _SIZE, _DTYPE = torch.Tensor.data_ptr, torch.Tensor.numel, attrgetter("dtype")
+_ADDRESS, _SIZE, _WHOLE = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_GRADIENT, _DTYPE = attrgetter("grad"), attrgetter("dtype")
 
 
 class AdamW:
@@ -164,22 +165,23 @@ class AdamW:
         by min(1, max_norm / (their norm + 1e-6)) on their way in, and the norm is returned (fp32 [],
         on the GPU; None without max_norm or where nothing has a gradient)."""
         params, sizes, dtypes = self.params, self._sizes, self._dtypes
-        grads = on = [p.grad for p in params]
+        grads = on = list(map(_GRADIENT, params))
         if any(g is None for g in grads):
             on = [g for g in grads if g is not None]
             if not on:
                 return None
-            sizes, dtypes = zip(*(c for *c, g in zip(sizes, dtypes, grads) if g is not None))
+            sizes, dtypes = map(list, zip(*(c for *c, g in zip(sizes, dtypes, grads) if g is not None)))
         # what a caller can have changed since the last step: data replaced or moved by p.data, the decays
         seen = (list(map(_ADDRESS, params)), [v.data_ptr() for v in self.state.values()], list(self.weight_decay))
         if self._words is None or seen != self._seen or list(map(_SIZE, params)) != self._sizes:
             self._fill()
             self._seen = seen
-        if list(map(_SIZE, on)) != list(sizes) or list(map(_DTYPE, on)) != list(dtypes):
+        if list(map(_SIZE, on)) != sizes or list(map(_DTYPE, on)) != dtypes:
             raise ValueError("a gradient must have its parameter's size and type")
-        whole = [g.contiguous() for g in on]  # alive until the launches are enqueued
-        addresses = list(map(_ADDRESS, whole))
-        if on is not grads:
+        if not all(map(_WHOLE, on)):
+            on = [g.contiguous() for g in on]  # alive until the launches are enqueued
+        addresses = list(map(_ADDRESS, on))
+        if len(on) != len(grads):
             left = iter(addresses)
             addresses = [0 if g is None else next(left) for g in grads]
         self._words[_GRAD::_FIELDS] = memoryview(array("Q", addresses))

@@ -6,8 +6,8 @@
 // The tensors are cut into chunks of whole groups of 256 values, a workgroup to a
 // chunk.  A launch's tensors lie in its arguments, which the host fills and a
 // captured graph keeps: no table is copied to the device.  Each wave finds its
-// chunk's tensor by comparing the chunk's number with all tensors' first chunks at
-// once, a lane each.
+// chunk's tensor by comparing the chunk's number with the tensors' first chunks, a
+// lane each.
 //
 // Three kinds of launches: the sums of the gradients' squares (with clipping
 // only), each workgroup's to a place of its own; one workgroup that adds them in
@@ -61,34 +61,47 @@ struct Factors {
 template <int BITS> struct Args {
     Entry<BITS> t[kEntries<BITS>];
     const Factors* f;
-    double* sums;  // of squares, a workgroup each
     float beta1, rest1, beta2, rest2, eps;
     int count;
     int64_t chunk;  // values, whole groups
 };
-static_assert(sizeof(Args<32>) <= 4000 && sizeof(Args<8>) <= 4000, "a launch's arguments");
+// The same of the sums of squares.
+struct Gradient {
+    int64_t n;
+    const void* g;
+    const void* p16;  // or null: fp32
+    int first;
+};
+constexpr int kGradients = 120;
+struct SquaresArgs {
+    Gradient t[kGradients];
+    double* sums;  // a workgroup each
+    int count;
+    int64_t chunk;
+};
+static_assert(sizeof(Args<32>) <= 4000 && sizeof(Args<8>) <= 4000 && sizeof(SquaresArgs) <= 4000, "a launch's arguments");
 
 // This workgroup's tensor, and its values from *from on up to *to.
-template <int BITS> __device__ __forceinline__ int place(const Args<BITS>& a, int64_t* from, int64_t* to) {
+template <typename A> __device__ __forceinline__ int place(const A& a, int64_t* from, int64_t* to) {
+    constexpr int most = (int)(sizeof(a.t) / sizeof(a.t[0]));
     const int lane = threadIdx.x & 63, b = (int)blockIdx.x;
-    const bool before = lane < a.count && a.t[lane < a.count ? lane : 0].first <= b;
-    const int i = __builtin_amdgcn_readfirstlane(__popcll(__ballot(before)) - 1);
+    int before = 0;
+#pragma unroll
+    for (int i = lane; i < (most + 63) / 64 * 64; i += 64)
+        before += __popcll(__ballot(i < a.count && a.t[i < a.count ? i : 0].first <= b));
+    const int i = __builtin_amdgcn_readfirstlane(before - 1);
     *from = (int64_t)(b - a.t[i].first) * a.chunk;
     *to = min(*from + a.chunk, a.t[i].n);
     return i;
 }
 
-// Four consecutive values as floats; zeros past `n`.
-__device__ __forceinline__ void load4(const Entry<32>& t, int64_t i, float* g) {
-    if (t.p16) load_part<bf16, 4>((const bf16*)t.g, i, t.n, g);
-    else load_part<float, 4>((const float*)t.g, i, t.n, g);
-}
-__device__ __forceinline__ void load4(const Entry<8>& t, int64_t i, float* g) {
+// Four consecutive gradients as floats; zeros past `n`.
+template <typename E> __device__ __forceinline__ void load4(const E& t, int64_t i, float* g) {
     if (t.p16) load_part<bf16, 4>((const bf16*)t.g, i, t.n, g);
     else load_part<float, 4>((const float*)t.g, i, t.n, g);
 }
 
-template <int BITS> __global__ __launch_bounds__(kThreads) void adamw_squares(Args<BITS> a) {
+__global__ __launch_bounds__(kThreads) void adamw_squares(SquaresArgs a) {
     __shared__ double s[kThreads];
     int64_t from, to;
     const int k = place(a, &from, &to);
@@ -253,13 +266,14 @@ void fill(Entry<8>& e, const mft_adamw_tensor& t) {
     e.m_scale = t.exp_avg_scale, e.v_scale = t.exp_avg_sq_scale;
     e.decay = (float)t.weight_decay;
 }
+void fill(Gradient& e, const mft_adamw_tensor& t) { e.n = t.n, e.g = t.grad, e.p16 = t.param_bf16; }
 bool steps(const mft_adamw_tensor& t) { return t.n > 0 && t.grad; }
 
 constexpr int64_t kSquares = 2048;  // workgroups of the sums of squares, but for one more a tensor
 
 // Launches over all tensors in chunks of `chunk` values: launch(args, workgroups).
-template <int BITS, typename F>
-void over(Args<BITS>& a, int32_t n, const mft_adamw_tensor* tensors, int64_t chunk, F launch) {
+template <typename A, typename F>
+void over(A& a, int32_t n, const mft_adamw_tensor* tensors, int64_t chunk, F launch) {
     a.chunk = chunk;
     a.count = 0;
     int64_t blocks = 0;
@@ -272,7 +286,7 @@ void over(Args<BITS>& a, int32_t n, const mft_adamw_tensor* tensors, int64_t chu
         fill(a.t[a.count], tensors[i]);
         a.t[a.count].first = (int)blocks;
         blocks += (tensors[i].n + chunk - 1) / chunk;
-        if (++a.count == kEntries<BITS>) flush();
+        if (++a.count == (int)(sizeof(a.t) / sizeof(a.t[0]))) flush();
     }
     flush();
 }
@@ -294,17 +308,19 @@ hipError_t run(const mft_adamw_desc& d, int32_t n, const mft_adamw_tensor* tenso
     a.eps = (float)d.eps;
     double* sums = reinterpret_cast<double*>(static_cast<char*>(workspace) + 256);
     int64_t count = 0;
-    if (d.max_norm > 0.0)
-        over<BITS>(a, n, tensors, whole((total + kSquares - 1) / kSquares, 4096), [&](Args<BITS>& q, unsigned blocks) {
+    if (d.max_norm > 0.0) {
+        SquaresArgs squares{};
+        over(squares, n, tensors, whole((total + kSquares - 1) / kSquares, 4096), [&](SquaresArgs& q, unsigned blocks) {
             q.sums = sums + count;
             count += blocks;
-            hipLaunchKernelGGL((adamw_squares<BITS>), dim3(blocks), dim3(kThreads), 0, st, q);
+            hipLaunchKernelGGL(adamw_squares, dim3(blocks), dim3(kThreads), 0, st, q);
         });
+    }
     StepArgs s{step, d.lr_device, d.lr, std::log(d.beta1), std::log(d.beta2), d.max_norm, sums, (int)count, norm,
                static_cast<Factors*>(workspace)};
     hipLaunchKernelGGL(adamw_factors, dim3(1), dim3(kStepThreads), 0, st, s);
     // 2^22 workgroups at most: a launch takes fewer than 2^32 threads
-    over<BITS>(a, n, tensors, whole((total >> 21) + 1, 2048), [&](Args<BITS>& q, unsigned blocks) {
+    over(a, n, tensors, whole((total >> 21) + 1, 2048), [&](Args<BITS>& q, unsigned blocks) {
         if constexpr (BITS == 32) hipLaunchKernelGGL(adamw_step32, dim3(blocks), dim3(kThreads), 0, st, q);
         else hipLaunchKernelGGL(adamw_step8, dim3(blocks), dim3(kThreads), 0, st, q);
     });
