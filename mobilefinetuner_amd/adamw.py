@@ -194,7 +194,7 @@ class AdamW:
             raise ValueError(f"max_norm must be positive, got {max_norm}")
         d = capi.adamw_desc(lr, *self.betas, self.eps, max_norm or 0.0, self.state_bits, address)
         with guard(params[0]):
-            norm = None if max_norm is None else torch.empty((), dtype=torch.float32, device=params[0].device)
+            norm = None if max_norm is None else params[0].new_empty((), dtype=torch.float32)
             ws = workspace(capi.adamw_workspace_size(d, self._table), params[0])
             capi.adamw_step(d, self._table, self.state["step"].data_ptr(), ptr(norm), ws.data_ptr(), stream(params[0]))
         torch.autograd.graph.increment_version(params)

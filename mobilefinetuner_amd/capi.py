@@ -1,5 +1,4 @@
-"""ctypes binding of the C ABI in ``include/mft/attention.h``,
-``include/mft/prologue.h`` and ``include/mft/lm_loss.h``.
+"""ctypes binding of the C ABI in ``include/mft/*.h``.
 
 This is the binding a Python caller would use (the C++ finetune_ops adapter
 links the same library directly).  It raises when the library is missing: the

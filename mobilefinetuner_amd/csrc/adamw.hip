@@ -1,7 +1,9 @@
 // One AdamW step over many tensors (C ABI in include/mft/adamw.h).
 //
 // Bound by memory: in fp32 28 bytes a value (the gradient and three values read,
-// three written), with 8-bit states and a bf16 parameter 16.
+// three written), with 8-bit states and a bf16 parameter 16.  A block's 27 M values in
+// fp32 127 us (6.0 TB/s, part of it from the last-level cache) and 36 for the sums of
+// squares; a bf16 table of 168 M with 8-bit states 498 us (5.4 TB/s).
 //
 // The tensors are cut into chunks of whole groups of 256 values, a workgroup to a
 // chunk.  A launch's tensors lie in its arguments, which the host fills and a
@@ -16,7 +18,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <vector>
 
 #include "attn_geometry.h"
 #include "attn_kernels.h"

@@ -88,7 +88,7 @@ def rows(t, last):
 
 
 def workspace(nbytes, like):
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 class _NoSecondDerivative(torch.autograd.Function):

@@ -43,7 +43,7 @@ def gated_linear(x, W_gate, W_up, activation="gelu_tanh", w_transposed=False, wa
     d, lead, n_ff = _desc(x, W_gate, W_up, activation, w_transposed)
     with guard(x):
         xc, Wg, Wu = x.contiguous(), W_gate.contiguous(), W_up.contiguous()
-        h = torch.empty(*lead, n_ff, dtype=x.dtype, device=x.device)
+        h = x.new_empty((*lead, n_ff))
         gate, up = (torch.empty_like(h), torch.empty_like(h)) if want_preact else (None, None)
         ws = workspace(capi.gated_linear_fwd_workspace_size(d), x)
         capi.gated_linear_fwd(d, xc.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), h.data_ptr(), ptr(gate), ptr(up), ptr(ws),
@@ -60,7 +60,7 @@ def gated_linear_e4m3(x, x_scale, W_gate, gate_scale, W_up, up_scale, activation
                                   (up_scale, "up_scale", (n_ff,)))]
     with guard(x):
         xc, Wg, Wu = x.contiguous(), W_gate.contiguous(), W_up.contiguous()
-        h = torch.empty(*lead, n_ff, dtype=torch.bfloat16, device=x.device)
+        h = x.new_empty((*lead, n_ff), dtype=torch.bfloat16)
         ws = workspace(capi.gated_linear_e4m3_workspace_size(d), x)
         capi.gated_linear_e4m3_fwd(d, xc.data_ptr(), scales[0].data_ptr(), Wg.data_ptr(), scales[1].data_ptr(),
                                    Wu.data_ptr(), scales[2].data_ptr(), h.data_ptr(), ptr(ws), stream(x))

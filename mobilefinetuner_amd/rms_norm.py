@@ -42,7 +42,7 @@ def rms_norm(x, weight=None, residual=None, norm="gemma", eps=1e-6):
     with guard(x):
         y = like(x)
         total = None if r2 is None else like(x)
-        rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
         d = capi.rms_norm_desc(x2.shape[0], D, DTYPES[x.dtype], how, eps, x2.stride(0),
                                0 if r2 is None else r2.stride(0))
         capi.rms_norm_fwd(d, x2.data_ptr(), ptr(r2), ptr(w), ptr(total), y.data_ptr(), rstd.data_ptr(), stream(x))
@@ -53,9 +53,9 @@ def _e4m3(x, weight, residual, how, eps):
     D, x2, r2 = _stream(x, residual)
     w = optional(weight, "weight", x, torch.float32, (D,))
     with guard(x):
-        q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+        q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
         total = None if r2 is None else like(x)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
         d = capi.rms_norm_desc(x2.shape[0], D, DTYPES[x.dtype], how, eps, x2.stride(0),
                                0 if r2 is None else r2.stride(0))
         capi.rms_norm_e4m3_fwd(d, x2.data_ptr(), ptr(r2), ptr(w), ptr(total), q.data_ptr(), scale.data_ptr(),
@@ -89,7 +89,7 @@ def rms_norm_backward(x, weight, rstd, dy, dtotal=None, norm="gemma", want_x=Tru
     rstd = operand(rstd, "rstd", x, torch.float32, x.shape[:-1]).contiguous()
     with guard(x):
         dx = like(x) if want_x else None
-        dw = torch.empty(D, dtype=torch.float32, device=x.device) if want_weight else None
+        dw = x.new_empty(D, dtype=torch.float32) if want_weight else None
         d = capi.rms_norm_desc(x2.shape[0], D, DTYPES[x.dtype], how, 0.0, x2.stride(0), 0, g2.stride(0),
                                0 if t2 is None else t2.stride(0))
         ws = workspace(capi.rms_norm_workspace_size(d), x)
