@@ -339,6 +339,14 @@ def test_offsets_past_32_bits(dev):
     for p, q in zip((dx[-40:], dWg, dWu), back):
         assert float((p - q).abs().max()) <= 2 * half(torch.bfloat16) * float(q.abs().max())
     del h, gate, up
+    args = [t.to(dev) for t in eight_bits(40, n_in, n_ff, 11, near=True)]
+    x8 = torch.zeros(N, n_in, dtype=torch.uint8, device=dev)
+    x8[-40:] = args[0].view(torch.uint8)
+    scale = torch.ones(N, device=dev)
+    scale[-40:] = args[1]
+    h = L.gated_linear_e4m3(x8.view(torch.float8_e4m3fn), scale, *args[2:])
+    assert torch.equal(h[-40:], L.gated_linear_e4m3(*args)) and (h[:100] == 0).all()  # sums that nothing rounds
+    del h, x8
 
 
 @pytest.mark.gpu
