@@ -81,6 +81,9 @@ class AdamW:
         self._words = None  # the C ABI's table of the tensors
         self.reload_masters()
 
+    def __getstate__(self):
+        return {**self.__dict__, "_words": None, "_table": None}  # addresses are a process's own
+
     @staticmethod
     def _places(sizes):
         at, starts = 0, []
@@ -178,7 +181,11 @@ class AdamW:
             self._seen = seen
         if list(map(_SIZE, on)) != sizes or list(map(_DTYPE, on)) != dtypes:
             raise ValueError("a gradient must have its parameter's size and type")
-        if not all(map(_WHOLE, on)):
+        try:
+            whole = all(map(_WHOLE, on))
+        except RuntimeError:
+            raise ValueError("a gradient must be dense") from None
+        if not whole:
             on = [g.contiguous() for g in on]  # alive until the launches are enqueued
         addresses = list(map(_ADDRESS, on))
         if len(on) != len(grads):

@@ -373,6 +373,29 @@ def test_what_a_caller_changes_between_steps(dev):
         y.backward()
 
 
+@pytest.mark.gpu
+def test_copies_and_gradient_modes(dev):
+    """A deep copy steps on its own; no_grad and inference_mode make no difference; states from host memory."""
+    import copy
+    from mobilefinetuner_amd.adamw import AdamW
+    opt = AdamW(make([300, 70], ["f32", "bf16"], 15), LR, state_bits=8)
+    opt.step(1.0)
+    other = copy.deepcopy(opt)
+    third = AdamW([p.detach().clone().requires_grad_(True) for p in opt.params], LR, state_bits=8)
+    third.load_state_dict({"state": {k: v.cpu() for k, v in opt.state_dict()["state"].items()}, "state_bits": 8})
+    for p, q, r in zip(opt.params, other.params, third.params):
+        assert p.data_ptr() != q.data_ptr() and torch.equal(p, q)
+        q.grad, r.grad = p.grad.clone(), p.grad.clone()
+    with torch.no_grad():
+        opt.step(1.0)
+    with torch.inference_mode():
+        other.step(1.0)
+    third.step(1.0)
+    for o in (other, third):
+        assert all(torch.equal(p, q) for p, q in zip(opt.params, o.params))
+        assert all(torch.equal(opt.state[k].float(), o.state[k].float()) for k in opt.state)
+
+
 # ------------------------------------------------------------------ refusals
 @pytest.fixture(scope="module")
 def capi():
@@ -458,6 +481,12 @@ def test_parameters_refused(dev):
         with pytest.raises(ValueError, match="lr"):
             opt.step()
     opt.lr = 1e-3
+    p.grad = None
+    p.grad = torch.eye(8, device=dev).to_sparse()
+    with pytest.raises(ValueError, match="dense"):
+        opt.step()
+    p.grad = None
+    p.grad = torch.zeros_like(p)
     p.data = torch.zeros(4, 8, device=dev)
     with pytest.raises(ValueError, match="size"):
         opt.step()

@@ -282,6 +282,26 @@ def test_leading_dimensions_and_other_layouts(dev, dtype):
 
 
 @pytest.mark.gpu
+def test_one_row_strided_numbers_and_one_weight_for_both(dev):
+    """x without leading dimensions, e4m3 numbers that are not contiguous, and gate and up by one trained weight,
+    whose gradient is the sum of both."""
+    from mobilefinetuner_amd import gated_linear as L
+    d = {k: v.to(dev) for k, v in make(3, 96, 40, "f32", 17).items()}
+    row = L.gated_linear(d["x"][0], d["W_gate"], d["W_up"])[0]
+    assert row.shape == (40,) and torch.equal(row, L.gated_linear(d["x"][:1], d["W_gate"], d["W_up"])[0][0])
+    q, qs, g, gs, u, us = (t.to(dev) for t in eight_bits(10, 96, 64, 18))
+    wide = torch.zeros(10, 192, dtype=torch.uint8, device=dev)
+    wide[:, ::2] = q.view(torch.uint8)
+    got = L.gated_linear_e4m3(wide.view(torch.float8_e4m3fn)[:, ::2], qs, g.t().contiguous().t(), gs, u, us)
+    assert torch.equal(got, L.gated_linear_e4m3(q, qs, g, gs, u, us))
+    W = d["W_gate"].clone().requires_grad_(True)
+    L.GatedLinear.apply(d["x"], W, W, "silu").backward(d["dh"])
+    _, gate, up = L.gated_linear(d["x"], W.detach(), W.detach(), "silu", False, True)
+    _, a, b = L.gated_linear_backward(d["x"], W.detach(), W.detach(), gate, up, d["dh"], "silu")
+    assert torch.equal(W.grad, a + b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_no_rows_and_parts_of_the_gradient(dev, dtype):
     from mobilefinetuner_amd import gated_linear as L

@@ -409,6 +409,32 @@ def test_captured_graph_follows_its_inputs(dev):
         assert all(torch.equal(p.float(), q.float()) for p, q in zip(held, step()))
 
 
+@pytest.mark.gpu
+def test_one_row_broadcast_rows_and_a_stream_added_to_itself(dev):
+    """x without leading dimensions, gradients of broadcast x, and x as its own residual: as by rows, by a
+    product of a copy, and twice one gradient."""
+    from mobilefinetuner_amd import rms_norm as L
+    x, r, w, dy, dt = (t.to(dev) for t in make(5, 96, "f32", 16))
+    rows, one = L.rms_norm(x, w, r), L.rms_norm(x[3], w, r[3])
+    assert one[2].shape == () and all(torch.equal(p[3], q) for p, q in zip(rows, one))
+    q, scale = L.quantize_rows(x[3])
+    assert q.shape == (96,) and scale.shape == () and torch.equal(q.float(), L.quantize_rows(x)[0][3].float())
+    dx, _ = L.rms_norm_backward(one[1], w, one[2], dy[3], dt[3])
+    assert torch.equal(dx, L.rms_norm_backward(rows[1], w, rows[2], dy, dt, want_weight=False)[0][3])
+    b = x[:1].clone().requires_grad_(True)
+    y, total = L.AddRMSNorm.apply(b.expand(5, 96), r, w)
+    torch.autograd.backward([y, total], [dy, dt])
+    c = x[:1].expand(5, 96).clone().requires_grad_(True)
+    y, total = L.AddRMSNorm.apply(c, r, w)
+    torch.autograd.backward([y, total], [dy, dt])
+    assert torch.equal(b.grad, c.grad.sum(0, keepdim=True))
+    s = x.clone().requires_grad_(True)
+    y, total = L.AddRMSNorm.apply(s, s, w)
+    torch.autograd.backward([y, total], [dy, dt])
+    _, total, rstd = L.rms_norm(x, w, x)
+    assert torch.equal(s.grad, 2 * L.rms_norm_backward(total, w, rstd, dy, dt)[0])
+
+
 # ------------------------------------------------------------------ refusals
 @pytest.fixture(scope="module")
 def capi():
