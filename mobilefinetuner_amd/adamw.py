@@ -181,11 +181,9 @@ class AdamW:
             self._seen = seen
         if list(map(_SIZE, on)) != sizes or list(map(_DTYPE, on)) != dtypes:
             raise ValueError("a gradient must have its parameter's size and type")
-        try:
-            whole = all(map(_WHOLE, on))
-        except RuntimeError:
-            raise ValueError("a gradient must be dense") from None
-        if not whole:
+        if not all(map(_WHOLE, on)):
+            if any(g.layout is not torch.strided for g in on):
+                raise ValueError("a gradient must be dense")
             on = [g.contiguous() for g in on]  # alive until the launches are enqueued
         addresses = list(map(_ADDRESS, on))
         if len(on) != len(grads):
