@@ -176,7 +176,8 @@ class AdamW:
             sizes, dtypes = map(list, zip(*(c for *c, g in zip(sizes, dtypes, grads) if g is not None)))
         # what a caller can have changed since the last step: data replaced or moved by p.data, the decays
         seen = (list(map(_ADDRESS, params)), [v.data_ptr() for v in self.state.values()], list(self.weight_decay))
-        if self._words is None or seen != self._seen or list(map(_SIZE, params)) != self._sizes:
+        if (self._words is None or seen != self._seen or list(map(_SIZE, params)) != self._sizes
+                or not all(map(_WHOLE, params))):
             self._fill()
             self._seen = seen
         if list(map(_SIZE, on)) != sizes or list(map(_DTYPE, on)) != dtypes:

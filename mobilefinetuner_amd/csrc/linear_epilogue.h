@@ -46,7 +46,7 @@ __device__ __forceinline__ void gated_epilogue(const LinearProduct& g, int64_t m
 // and the columns' gs and us scale the sums (SCALED: e4m3).  Where no vector of V is
 // cut by the rows' end and the activation is smooth, which the whole launch shares, the
 // columns take the short way: the matrix units wait meanwhile.  8192 x 1152 -> 6912 on
-// 256 x 256 tiles 345 us with a choice and an end for each column, 293 by this.
+// 256 x 256 tiles 345 us with a choice and an end for each column, 267 by this.
 template <int COLS, int PITCH, bool SCALED>
 __device__ __forceinline__ void gated_rows_out(const LinearProduct& g, int64_t mw, int64_t nw, const float* st, int lane,
                                                const float* xs, const float* gs, const float* us) {

@@ -495,3 +495,23 @@ def test_parameters_refused(dev):
     with pytest.raises(ValueError, match="exp_avg"):
         opt.step()
     assert int(opt.state["step"]) == 0
+
+
+@pytest.mark.gpu
+def test_parameters_turned_in_place_refused(dev):
+    from mobilefinetuner_amd.adamw import AdamW
+    p = torch.randn(8, 4, device=dev, requires_grad=True)
+    opt = AdamW([p])
+    p.grad = torch.randn_like(p)
+    opt.step()
+    before = p.detach().clone()
+    p.grad = None
+    p.data = p.data.t()  # the same memory and size in another order
+    p.grad = torch.ones(4, 8, device=dev)
+    with pytest.raises(ValueError, match="contiguous"):
+        opt.step()
+    assert int(opt.state["step"]) == 1 and torch.equal(p.detach().t(), before)
+    p.data = p.data.t()
+    p.grad = torch.ones(8, 4, device=dev)
+    opt.step()
+    assert int(opt.state["step"]) == 2 and not torch.equal(p.detach(), before)
