@@ -168,12 +168,13 @@ class AdamW:
         by min(1, max_norm / (their norm + 1e-6)) on their way in, and the norm is returned (fp32 [],
         on the GPU; None without max_norm or where nothing has a gradient)."""
         params, sizes, dtypes = self.params, self._sizes, self._dtypes
+        stepped = params
         grads = on = list(map(_GRADIENT, params))
         if any(g is None for g in grads):
             on = [g for g in grads if g is not None]
             if not on:
                 return None
-            sizes, dtypes = map(list, zip(*(c for *c, g in zip(sizes, dtypes, grads) if g is not None)))
+            sizes, dtypes, stepped = map(list, zip(*(c for *c, g in zip(sizes, dtypes, params, grads) if g is not None)))
         # what a caller can have changed since the last step: data replaced or moved by p.data, the decays
         seen = (list(map(_ADDRESS, params)), [v.data_ptr() for v in self.state.values()], list(self.weight_decay))
         if (self._words is None or seen != self._seen or list(map(_SIZE, params)) != self._sizes
@@ -203,5 +204,5 @@ class AdamW:
             norm = None if max_norm is None else params[0].new_empty((), dtype=torch.float32)
             ws = workspace(capi.adamw_workspace_size(d, self._table), params[0])
             capi.adamw_step(d, self._table, self.state["step"].data_ptr(), ptr(norm), ws.data_ptr(), stream(params[0]))
-        torch.autograd.graph.increment_version(params)
+        torch.autograd.graph.increment_version(stepped)
         return norm

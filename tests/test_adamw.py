@@ -515,3 +515,19 @@ def test_parameters_turned_in_place_refused(dev):
     p.grad = torch.ones(8, 4, device=dev)
     opt.step()
     assert int(opt.state["step"]) == 2 and not torch.equal(p.detach(), before)
+
+
+@pytest.mark.gpu
+def test_a_pending_backward_through_what_is_not_stepped(dev):
+    from mobilefinetuner_amd.adamw import AdamW
+    p, q = (torch.full((8,), v, device=dev, requires_grad=True) for v in (2.0, 3.0))
+    opt = AdamW([p, q])
+    loss = (q * q).sum()  # holds q until its backward
+    p.grad = torch.ones_like(p)
+    opt.step()
+    loss.backward()
+    assert torch.equal(q.grad, torch.full_like(q, 6.0))
+    loss = (p * p).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
