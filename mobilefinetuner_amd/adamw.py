@@ -166,7 +166,7 @@ class AdamW:
     def step(self, max_norm=None):
         """One step of the parameters that have a gradient.  With max_norm all gradients are scaled
         by min(1, max_norm / (their norm + 1e-6)) on their way in, and the norm is returned (fp32 [],
-        on the GPU; None without max_norm or where nothing has a gradient)."""
+        on the GPU; None without max_norm or where no value has a gradient)."""
         params, sizes, dtypes = self.params, self._sizes, self._dtypes
         stepped = params
         grads = on = list(map(_GRADIENT, params))
@@ -175,6 +175,8 @@ class AdamW:
             if not on:
                 return None
             sizes, dtypes, stepped = map(list, zip(*(c for *c, g in zip(sizes, dtypes, params, grads) if g is not None)))
+        if not any(sizes):
+            return None
         # what a caller can have changed since the last step: data replaced or moved by p.data, the decays
         seen = (list(map(_ADDRESS, params)), [v.data_ptr() for v in self.state.values()], list(self.weight_decay))
         if (self._words is None or seen != self._seen or list(map(_SIZE, params)) != self._sizes

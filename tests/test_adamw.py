@@ -531,3 +531,15 @@ def test_a_pending_backward_through_what_is_not_stepped(dev):
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_nothing_but_empty_gradients(dev, bits):
+    from mobilefinetuner_amd.adamw import AdamW
+    p, q = torch.zeros(0, 4, device=dev, requires_grad=True), torch.ones(4, device=dev, requires_grad=True)
+    for params in ([p], [p, q]):
+        opt = AdamW(params, state_bits=bits)
+        p.grad = torch.zeros_like(p)
+        assert opt.step(1.0) is None and opt.step() is None
+        assert int(opt.state["step"]) == 0 and torch.equal(q.detach(), torch.ones_like(q))
