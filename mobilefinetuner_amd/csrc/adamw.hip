@@ -244,13 +244,13 @@ __global__ __launch_bounds__(kThreads) void adamw_step8(Args<8> a) {
         const float ms = e4m3_scale(wave_max_u(most_m, lane)), rs = e4m3_scale(wave_max_u(most_r, lane));
         if (lane == 0) t.m_scale[group] = ms, t.v_scale[group] = rs;
         if (i >= t.n) continue;
-        const float mi = 1.f / ms, ri = 1.f / rs;
+        bool some[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[e] *= mi;
-            const float q = r[e] * ri;
-            r[e] = r[e] > 0.f && q < kE4m3Min ? kE4m3Min : q;
-        }
+        for (int e = 0; e < 4; ++e) some[e] = r[e] > 0.f;
+        E4m3Divisor(ms).divide<4>(x);
+        E4m3Divisor(rs).divide<4>(r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = some[e] && r[e] < kE4m3Min ? kE4m3Min : r[e];
         e4m3_store<4>(mq + i, t.n - i, x);
         e4m3_store<4>(vq + i, t.n - i, r);
         store_part<float, 4>(t.p, i, t.n, p);

@@ -20,6 +20,32 @@ __device__ __forceinline__ float e4m3_scale(uint32_t max_bits) {
     return s < kScaleMin ? kScaleMin : s;  // a NaN stays
 }
 
+// Quotients by a scale, each x / scale rounded to nearest once, of which e4m3 numbers are then taken: by the
+// reciprocal alone (x inv) 0.06 percent of a bf16 matrix's came out a number off, as its quotients often lie halfway
+// between two.  Two corrections by exact remainders: the first leaves a number next to the quotient, and from there
+// the second rounds it correctly (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990: inv is the nearest to 1 / scale, the remainder a float).  The remainder of a quotient from 2^-11 on
+// is a float while the scale is above 2^-91; smaller quotients are zeros either way.  An infinite scale's finite values
+// are 0.  8192 x 1152 with its norm 17.0 us, by the reciprocal 16.3, by the operator's own sequence throughout 18.6.
+struct E4m3Divisor {
+    float scale, inv;
+    bool fast;
+    __device__ __forceinline__ explicit E4m3Divisor(float s) : scale(s), inv(1.0f / s), fast(s >= 0x1p-80f && s < INFINITY) {}
+    template <int V> __device__ __forceinline__ void divide(float* x) const {
+        if (fast) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                float q = x[e] * inv;
+                q = fmaf(fmaf(-q, scale, x[e]), inv, q);
+                x[e] = fmaf(fmaf(-q, scale, x[e]), inv, q);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] /= scale;
+        }
+    }
+};
+
 // Four values to nearest even.  Up to 448 (1 + 2^-23), which rounds to 448: no
 // value of a group exceeds its scale's by more.
 __device__ __forceinline__ uint32_t e4m3_pack4(float a, float b, float c, float d) {

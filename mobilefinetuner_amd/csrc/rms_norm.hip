@@ -132,14 +132,14 @@ __global__ __launch_bounds__(kThreads<WPR>) void rms_fwd(RmsNormArgs a) {
         }
     }
     if constexpr (E4M3) {
-        const float scale = e4m3_scale(row_max<WPR>(top, s2)), inv = 1.0f / scale;
+        const float scale = e4m3_scale(row_max<WPR>(top, s2));
+        const E4m3Divisor by(scale);
         if (t == 0) a.scale[n] = scale;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int64_t d0 = (int64_t)(c * TPR + t) * V;
             if (d0 >= a.D) break;
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[c][e] *= inv;
+            by.divide<V>(x[c]);
             e4m3_store<V>((uint8_t*)a.y + n * a.sy + d0, a.D - d0, x[c]);
         }
     }
@@ -175,7 +175,7 @@ template <typename T, bool E4M3> __global__ __launch_bounds__(kLongThreads) void
 #pragma unroll
         for (int e = 0; e < V; ++e) x[e] = x[e] * rstd * f[e];
     };
-    float inv = 1.f;
+    float scale = 1.f;
     if constexpr (E4M3) {
         uint32_t top = 0;
         for (int64_t d0 = first; d0 < a.D; d0 += STEP) {
@@ -185,16 +185,15 @@ template <typename T, bool E4M3> __global__ __launch_bounds__(kLongThreads) void
             for (int e = 0; e < V; ++e)
                 if (d0 + e < a.D) top = max(top, magnitude(x[e]));
         }
-        const float scale = e4m3_scale(row_max<kLongWaves>(top, s2));
+        scale = e4m3_scale(row_max<kLongWaves>(top, s2));
         if (threadIdx.x == 0) a.scale[n] = scale;
-        inv = 1.0f / scale;
     }
+    const E4m3Divisor by(scale);
     for (int64_t d0 = first; d0 < a.D; d0 += STEP) {
         float x[V];
         values(d0, x);
         if constexpr (E4M3) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[e] *= inv;
+            by.divide<V>(x);
             e4m3_store<V>((uint8_t*)a.y + n * a.sy + d0, a.D - d0, x);
         } else {
             store_part<T, V>((T*)a.y + n * a.sy, d0, a.D, x);

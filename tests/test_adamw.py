@@ -543,3 +543,29 @@ def test_nothing_but_empty_gradients(dev, bits):
         p.grad = torch.zeros_like(p)
         assert opt.step(1.0) is None and opt.step() is None
         assert int(opt.state["step"]) == 0 and torch.equal(q.detach(), torch.ones_like(q))
+
+
+@pytest.mark.gpu
+def test_eight_bits_are_those_of_the_quotient(dev):
+    """To the bit, scale = max |x| / 448 and q = e4m3(x / scale), both quotients in fp32, for x = m and sqrt(v): those
+    of a first step are (1 - beta1) g and sqrt((1 - beta2) g^2), as with states in 32 bits.  Gradients with few
+    digits, whose quotients often lie halfway between two numbers."""
+    from mobilefinetuner_amd.adamw import AdamW
+    g = torch.Generator().manual_seed(21)
+    grad = (torch.randint(1, 256, (1 << 18,), generator=g) / 128 * (1 - 2 * torch.randint(0, 2, (1 << 18,), generator=g)))
+    grad *= 2.0 ** torch.randint(-6, 1, (1 << 18,), generator=g)
+    opts = []
+    for bits in (32, 8):
+        p = torch.zeros(1 << 18, device=dev, requires_grad=True)
+        p.grad = grad.to(dev)
+        opts.append(AdamW([p], LR, (0.5, 0.75), EPS, state_bits=bits))  # powers of two: m and v have few digits, too
+        opts[-1].step()
+    wide, narrow = (o.state for o in opts)
+    for name, x in (("exp_avg", wide["exp_avg"].cpu()), ("exp_avg_sq", wide["exp_avg_sq"].cpu().sqrt())):
+        x = x.view(-1, 256)
+        scale = x.abs().amax(1) / torch.tensor(448.0)
+        assert torch.equal(narrow[name + "_scale"].cpu(), scale)
+        q = (x / scale[:, None]).to(torch.float8_e4m3fn).float()
+        if name == "exp_avg_sq":
+            q = torch.where(x > 0, q.clamp(min=2.0 ** -9), q)
+        assert torch.equal(narrow[name].float().cpu().view(-1, 256), q)
