@@ -59,8 +59,9 @@ mft_status mft_gated_linear_fwd(const mft_gated_linear_desc* desc, const void* x
                                 void* h, void* gate, void* up, void* workspace, hipStream_t stream);
 
 /* dx, dW_gate and dW_up, each left out where NULL, written and not accumulated.  x
- * may be NULL without the weights' gradients, the weights without dx.  fp32
- * gradients stored [ff, in] with dW_up right behind dW_gate are one product. */
+ * may be NULL without the weights' gradients, the weights without dx.  Both weights'
+ * gradients in fp32 stored [ff, in] are one product: one of them alone can differ from
+ * it in its rounding. */
 mft_status mft_gated_linear_bwd(const mft_gated_linear_desc* desc, const void* x, const void* W_gate, const void* W_up,
                                 const void* gate, const void* up, const void* dh, void* dx, void* dW_gate, void* dW_up,
                                 void* workspace, hipStream_t stream);

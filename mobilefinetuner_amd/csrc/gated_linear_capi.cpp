@@ -106,8 +106,7 @@ FwdLayout fwd_layout(const mft_gated_linear_desc* d) {
     l.total = l.gemm + mft::gemm_f32_workspace(f_fwd(d));
     return l;
 }
-// fp32: one product for both weights' gradients where they lie one behind the other, stored [ff, in].  Twice the
-// tiles at once: 509 x 640 -> 2048 31 us against 45 (bf16 at 4096 x 1152 -> 6912, whose single products fill the
+// fp32: one product for both weights' gradients stored [ff, in], each to its own memory.  Twice the tiles at once: 509 x 640 -> 2048 31 us against 45 (bf16 at 4096 x 1152 -> 6912, whose single products fill the
 // GPU: 341 us of a backward against 338).
 bool may_be_both(const mft_gated_linear_desc* d) { return !is_bf(d) && d->w_transposed; }
 
@@ -233,8 +232,7 @@ mft_status mft_gated_linear_bwd(const mft_gated_linear_desc* desc, const void* x
             }
         }
     }
-    const bool both = may_be_both(desc) && dW_gate &&
-                      dW_up == static_cast<float*>(dW_gate) + desc->in_dim * desc->ff_dim;
+    const bool both = may_be_both(desc) && dW_gate && dW_up;
     for (int i = 0; i < (both ? 1 : 2) && e == hipSuccess; ++i) {
         if (!dW[i]) continue;
         const void* rows = desc->w_transposed ? dz[i] : x;
@@ -247,6 +245,7 @@ mft_status mft_gated_linear_bwd(const mft_gated_linear_desc* desc, const void* x
             mft::GemmF32 g = f_dw(desc, both);
             g.terms[0].A = static_cast<const float*>(rows), g.terms[0].B = static_cast<const float*>(cols);
             g.C = static_cast<float*>(dW[i]), g.partial = sums;
+            if (both) g.C2 = static_cast<float*>(dW_up), g.rows = desc->ff_dim;
             e = mft::launch_gemm_f32(g, stream);
         }
     }

@@ -480,7 +480,10 @@ __global__ __launch_bounds__(256 * KW, 3) void gemm_f32_kernel(Args a) {
     float* C = a.whole ? a.g.C : a.g.partial + (int64_t)slice * a.g.M * a.g.N;
     const int64_t ldc = a.whole ? a.g.ldc : a.g.N;
     const float* bias = a.whole ? a.g.bias : nullptr;
-    const bool vec = ldc % 4 == 0 && reinterpret_cast<uintptr_t>(C) % 16 == 0;
+    // Elements from where a row of C2 would lie in C to where it lies.
+    const int64_t away = a.whole && a.g.C2 ? (int64_t)(reinterpret_cast<intptr_t>(a.g.C2) - reinterpret_cast<intptr_t>(C)) / 4 - a.g.rows * ldc : 0;
+    const int64_t second = a.whole && a.g.C2 ? a.g.rows : a.g.M;
+    const bool vec = ldc % 4 == 0 && reinterpret_cast<uintptr_t>(C) % 16 == 0 && away % 4 == 0;
     const int64_t mw = m0 + wm * (TM / 2) + n2, nw = n0 + wn * (TN / 2) + 4 * hh2;
     if (a.whole && a.g.add) {  // all of C's loads ahead of the stores
 #pragma unroll
@@ -520,7 +523,7 @@ __global__ __launch_bounds__(256 * KW, 3) void gemm_f32_kernel(Args a) {
                         continue;
                     }
                 }
-                float* d = C + m * ldc + c0;
+                float* d = C + m * ldc + (m < second ? 0 : away) + c0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (bias && c0 + e < a.g.N) o[e] += bias[c0 + e];
@@ -552,7 +555,7 @@ __global__ __launch_bounds__(256) void gemm_f32_reduce(Args a) {
         run_epilogue<VEC>(a.g, m, n, v);
         return;
     }
-    float* d = a.g.C + m * a.g.ldc + n;
+    float* d = a.g.C2 && m >= a.g.rows ? a.g.C2 + (m - a.g.rows) * a.g.ldc + n : a.g.C + m * a.g.ldc + n;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) d[e] = sum[e] + (a.g.bias ? a.g.bias[n + e] : 0.f) + (a.g.add ? d[e] : 0.f);
 }
@@ -636,7 +639,8 @@ size_t gemm_f32_workspace(const GemmF32& g) {
 
 hipError_t launch_gemm_f32(const GemmF32& g, hipStream_t st) {
     if (g.M <= 0 || g.N <= 0) return hipSuccess;
-    if (with_epilogue(g) && (g.ldc != g.N || g.terms[0].ta || g.add)) return hipErrorInvalidValue;
+    if (with_epilogue(g) && (g.ldc != g.N || g.terms[0].ta || g.add || g.C2)) return hipErrorInvalidValue;
+    if (g.C2 && g.add) return hipErrorInvalidValue;
     const Plan p = plan(g);
     if (p.small)
         launch_t<64, 32, 2>(p.a, st);

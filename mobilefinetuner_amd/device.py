@@ -37,18 +37,6 @@ def like(t):
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def pair_like(t):
-    """Two new contiguous tensors of t's shape and type, one behind the other in memory (tensors of their
-    own, not views)."""
-    n = t.numel()
-    both = torch.empty(2 * n, dtype=t.dtype, device=t.device).untyped_storage()
-    strides = [1]
-    for d in reversed(t.shape[1:]):
-        strides.append(strides[-1] * d)
-    return tuple(torch.empty(0, dtype=t.dtype, device=t.device).set_(both, i * n, t.shape, strides[::-1])
-                 for i in range(2))
-
-
 def ptr(t):
     return None if t is None else t.data_ptr()
 

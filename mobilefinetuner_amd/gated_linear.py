@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from . import capi
-from .device import DTYPES, first_order, guard, like, operand, pair_like, ptr, stream, workspace
+from .device import DTYPES, first_order, guard, like, operand, ptr, stream, workspace
 
 ACTIVATIONS = {"relu": capi.MFT_ACT_RELU, "gelu_tanh": capi.MFT_ACT_GELU_TANH, "silu": capi.MFT_ACT_SILU}
 
@@ -77,10 +77,7 @@ def gated_linear_backward(x, W_gate, W_up, gate, up, dh, activation="gelu_tanh",
     with guard(x):
         xc, Wg, Wu = x.contiguous(), W_gate.contiguous(), W_up.contiguous()
         dx = like(x) if want_x else None
-        if want_gate and want_up and w_transposed and x.dtype == torch.float32:  # one product for both
-            dWg, dWu = pair_like(W_gate)
-        else:
-            dWg, dWu = like(W_gate) if want_gate else None, like(W_up) if want_up else None
+        dWg, dWu = like(W_gate) if want_gate else None, like(W_up) if want_up else None
         ws = workspace(capi.gated_linear_workspace_size(d)[1], x)
         capi.gated_linear_bwd(d, xc.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), gate.data_ptr(), up.data_ptr(),
                               dh.data_ptr(), ptr(dx), ptr(dWg), ptr(dWu), ptr(ws), stream(x))

@@ -537,3 +537,28 @@ def test_operands_that_do_not_fit_refused(dev):
                 lambda: L.gated_linear_e4m3(q, s, w, ws, w, ws.bfloat16()), lambda: L.gated_linear(q, w, w)):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(40, 72, 48), (33, 65, 51), (509, 640, 2048)], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_have_memory_of_their_own(dev, shape):
+    """Each weight's gradient alone in its storage, and the same bits wherever the caller's buffers lie: one behind
+    the other, apart, in the other order, off 16 bytes."""
+    from mobilefinetuner_amd import capi
+    from mobilefinetuner_amd import gated_linear as L
+    print(f"[case] {shape}", flush=True)
+    N, n_in, n_ff = shape
+    n = n_ff * n_in
+    d = {k: v.to(dev) for k, v in make(*shape, "f32", 19, True).items()}
+    args = [d[k] for k in ("x", "W_gate", "W_up", "gate", "up", "dh")]
+    _, a, b = L.gated_linear_backward(*args, w_transposed=True)
+    for g in (a, b):
+        assert g.untyped_storage().nbytes() == 4 * n and g.storage_offset() == 0
+    desc = capi.gated_linear_desc(N, n_in, n_ff, w_transposed=True)
+    ws = torch.empty(capi.gated_linear_workspace_size(desc)[1], dtype=torch.uint8, device=dev)
+    for at, too in ((0, n), (0, n + 64), (n + 64, 0), (0, n + 1), (3, n + 8)):
+        out = torch.full((2 * n + 128,), math.nan, device=dev)
+        capi.gated_linear_bwd(desc, *(t.data_ptr() for t in args), None, out.data_ptr() + 4 * at, out.data_ptr() + 4 * too,
+                              ws.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(out[at : at + n], a.view(-1)) and torch.equal(out[too : too + n], b.view(-1))
+        assert int(out.isnan().sum()) == 128  # nothing else is written
