@@ -552,8 +552,8 @@ def test_gradients_have_memory_of_their_own(dev, shape):
     d = {k: v.to(dev) for k, v in make(*shape, "f32", 19, True).items()}
     args = [d[k] for k in ("x", "W_gate", "W_up", "gate", "up", "dh")]
     _, a, b = L.gated_linear_backward(*args, w_transposed=True)
-    for g in (a, b):
-        assert g.untyped_storage().nbytes() == 4 * n and g.storage_offset() == 0
+    held = [(g.untyped_storage().nbytes(), g.storage_offset()) for g in (a, b)]
+    assert held == [(4 * n, 0)] * 2
     desc = capi.gated_linear_desc(N, n_in, n_ff, w_transposed=True)
     ws = torch.empty(capi.gated_linear_workspace_size(desc)[1], dtype=torch.uint8, device=dev)
     for at, too in ((0, n), (0, n + 64), (n + 64, 0), (0, n + 1), (3, n + 8)):
