@@ -123,10 +123,16 @@ class AdamW:
                 p.grad.zero_()
 
     def state_dict(self):
-        return {"state": {k: v.clone() for k, v in self.state.items()}, "state_bits": self.state_bits}
+        return {"state": {k: v.clone() for k, v in self.state.items()}, "state_bits": self.state_bits,
+                "params": self._parts()}
+
+    def _parts(self):
+        """Whose the flat states' parts are: each parameter's shape and type."""
+        return [(list(p.shape), str(t)) for p, t in zip(self.params, self._dtypes)]
 
     def load_state_dict(self, d):
-        """Takes over a copy of another's state; the parameters are the caller's to load, before or after."""
+        """Takes over a copy of another's state; the parameters are the caller's to load, before or after.  They
+        must have the other's shapes and types, in its order (what a state without "params" does not tell)."""
         state = d["state"]
         if d["state_bits"] != self.state_bits or state.keys() != self.state.keys():
             raise ValueError(f"the state has {d['state_bits']} bits and {sorted(state)}, "
@@ -134,6 +140,12 @@ class AdamW:
         for k, (shape, dtype) in self._layout.items():
             if state[k].shape != shape or state[k].dtype != dtype:
                 raise ValueError(f"{k} must be {dtype} {list(shape)}, got {state[k].dtype} {list(state[k].shape)}")
+        if "params" in d:
+            given, own = [(list(s), t) for s, t in d["params"]], self._parts()
+            if given != own:
+                i = next((i for i, (a, b) in enumerate(zip(given, own)) if a != b), min(len(given), len(own)))
+                raise ValueError(f"the state is of {len(given)} parameters, this optimizer has {len(own)}: they differ "
+                                 f"from parameter {i} on, {given[i:i + 1]} and {own[i:i + 1]}")
         for k, v in state.items():
             self.state[k].copy_(v)
 

@@ -569,3 +569,35 @@ def test_eight_bits_are_those_of_the_quotient(dev):
         if name == "exp_avg_sq":
             q = torch.where(x > 0, q.clamp(min=2.0 ** -9), q)
         assert torch.equal(narrow[name].float().cpu().view(-1, 256), q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_of_other_parameters_refused(dev, bits, tmp_path):
+    """The same padded size in other parts: swapped, cut elsewhere, turned, the master beside the other parameter.  A
+    state without the parameters' shapes loads as far as its sizes fit."""
+    from mobilefinetuner_amd.adamw import AdamW
+
+    def opt(*params):
+        ps = [torch.ones(s, device=dev, dtype=t).requires_grad_(True) for s, t in params]
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        return AdamW(ps, state_bits=bits)
+
+    f, b = torch.float32, torch.bfloat16
+    first = opt(([300], f), ([200], f), ([16, 8], b), ([8, 16], f))
+    first.step()
+    torch.save(first.state_dict(), tmp_path / "state")
+    saved = torch.load(tmp_path / "state", weights_only=True)
+    for others in ([([200], f), ([300], f), ([16, 8], b), ([8, 16], f)], [([301], f), ([199], f), ([16, 8], b), ([8, 16], f)],
+                   [([300], f), ([200], f), ([8, 16], b), ([8, 16], f)], [([300], f), ([200], f), ([16, 8], f), ([8, 16], b)],
+                   [([300], f), ([200], f), ([16, 8], b), ([8, 16], f), ([0], f)], [([500], f), ([16, 8], b), ([8, 16], f)]):
+        other = opt(*others)
+        before = {k: v.clone() for k, v in other.state.items()}
+        with pytest.raises(ValueError, match="they differ|must be"):
+            other.load_state_dict(saved)
+        assert all(torch.equal(before[k].float(), v.float()) for k, v in other.state.items())
+    for d in (saved, {k: saved[k] for k in ("state", "state_bits")}):
+        same = opt(([300], f), ([200], f), ([16, 8], b), ([8, 16], f))
+        same.load_state_dict(d)
+        assert all(torch.equal(first.state[k].float(), v.float()) for k, v in same.state.items())
