@@ -55,10 +55,7 @@ class AdamW:
         if any(a[1] > b[0] for a, b in zip(ends, ends[1:])):
             raise ValueError("a parameter is given twice, or shares memory with another")
         self.lr, self.betas, self.eps = lr, tuple(betas), eps
-        decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(self.params)
-        if len(decay) != len(self.params):
-            raise ValueError(f"weight_decay has {len(decay)} values for {len(self.params)} parameters")
-        self.weight_decay, self.state_bits = decay, state_bits
+        self.weight_decay, self.state_bits = weight_decay, state_bits
         self._sizes = [p.numel() for p in self.params]
         half = [p.dtype == torch.bfloat16 for p in self.params]
         self._dtypes = [p.dtype for p in self.params]
@@ -80,6 +77,21 @@ class AdamW:
         self._layout = {k: (v.shape, v.dtype) for k, v in self.state.items()}
         self._words = None  # the C ABI's table of the tensors
         self.reload_masters()
+
+    @property
+    def weight_decay(self):
+        """A list of one for each parameter."""
+        return self.__dict__["weight_decay"]
+
+    @weight_decay.setter
+    def weight_decay(self, decay):
+        decay = list(decay) if isinstance(decay, (list, tuple)) else [decay] * len(self.params)
+        self.__dict__["weight_decay"] = self._one_each(decay)
+
+    def _one_each(self, decay):
+        if len(decay) != len(self.params):
+            raise ValueError(f"weight_decay has {len(decay)} values for {len(self.params)} parameters")
+        return decay
 
     def __getstate__(self):
         return {**self.__dict__, "_words": None, "_table": None}  # addresses are a process's own
@@ -152,6 +164,7 @@ class AdamW:
     def _fill(self):
         """The C ABI's table of the tensors, but for their gradients."""
         params, first = self.params, self.params[0]
+        decay = self._one_each(self.weight_decay)
         for p, n, t in zip(params, self._sizes, self._dtypes):
             operand(p, "a parameter", first, t)
             if p.numel() != n or not p.is_contiguous():
@@ -171,7 +184,7 @@ class AdamW:
             if self.state_bits == 8:
                 t.exp_avg_scale = at["exp_avg_scale"] + 4 * (a // GROUP)
                 t.exp_avg_sq_scale = at["exp_avg_sq_scale"] + 4 * (a // GROUP)
-            t.weight_decay = self.weight_decay[i]
+            t.weight_decay = decay[i]
         self._table = (capi.AdamWTensor * len(params)).from_buffer(table)
         self._words = memoryview(table).cast("Q")
 

@@ -601,3 +601,31 @@ def test_states_of_other_parameters_refused(dev, bits, tmp_path):
         same = opt(([300], f), ([200], f), ([16, 8], b), ([8, 16], f))
         same.load_state_dict(d)
         assert all(torch.equal(first.state[k].float(), v.float()) for k, v in same.state.items())
+
+
+@pytest.mark.gpu
+def test_weight_decay_set_between_steps(dev):
+    """A number, a list or one element of it, as at the start; lists of another length are refused and nothing is
+    stepped."""
+    params = make([100, 200, 300], ["f32", "bf16", "f32"], 10)
+    opt = run(params, weight_decay=0.3)
+    t = 2
+    for decay in (0.1, [0.0, 0.2, 0.4], (0.5, 0.6, 0.7)):
+        opt.weight_decay = decay
+        assert opt.weight_decay == (list(decay) if isinstance(decay, (list, tuple)) else [decay] * 3)
+        before, t = snapshot(opt), t + 1
+        opt.step()
+        check(opt, before, t, None, None)
+    opt.weight_decay[1] = 5.0
+    before, t = snapshot(opt), t + 1
+    opt.step()
+    check(opt, before, t, None, None)
+    for decay in ([0.1], [0.1] * 4, []):
+        with pytest.raises(ValueError, match="weight_decay has"):
+            opt.weight_decay = decay
+    before = snapshot(opt)
+    for change in (lambda: opt.weight_decay.append(0.1), lambda: [opt.weight_decay.pop() for _ in range(2)]):
+        change()
+        with pytest.raises(ValueError, match="weight_decay has"):
+            opt.step()
+    assert int(opt.state["step"]) == t and all(torch.equal(a[k], b[k]) for a, b in zip(before, snapshot(opt)) for k in "pmv")
