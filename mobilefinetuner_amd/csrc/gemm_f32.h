@@ -35,7 +35,8 @@ struct GemmF32 {
     float* z;
     // The gated linear layer's, with the same: z is the sum, C = act(gate) times it; no bias or residual.
     const float* gate;  // [M, N] or null
-    // Rows of C from `rows` on, in memory of their own (null: none), with the same row stride; no add, no epilogue.
+    // Rows of C from `rows` on, in memory of their own (null: none), with the same row stride: A stored [K, M], B
+    // [K, N], no add and no epilogue.
     float* C2;
     int64_t rows;
 };

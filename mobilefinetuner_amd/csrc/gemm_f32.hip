@@ -212,9 +212,12 @@ template <int VEC> __device__ __forceinline__ void run_epilogue(const GemmF32& g
     }
 }
 
-// TA / TB: term 0's storage.  EPI: with the linear layer's epilogue.  KW groups of 2 x 2 waves share a stage's 16-deep
+// What the sums go to: C, C and C2, or the linear or gated layer's epilogue.
+enum { TO_C, TO_BOTH, TO_EPILOGUE };
+
+// TA / TB: term 0's storage.  OUT: where its sums go.  KW groups of 2 x 2 waves share a stage's 16-deep
 // k steps; their accumulators are added through LDS at the end.
-template <int T, int BK, int KW, bool TA, bool TB, bool EPI>
+template <int T, int BK, int KW, bool TA, bool TB, int OUT>
 __global__ __launch_bounds__(256 * KW, 3) void gemm_f32_kernel(Args a) {
     constexpr int MT = T / 64, NT = T / 64;  // 32 x 32 tiles per wave
     constexpr int kThreads = 256 * KW, KS = BK / 16 / KW;  // k steps of a wave per stage
@@ -480,10 +483,9 @@ __global__ __launch_bounds__(256 * KW, 3) void gemm_f32_kernel(Args a) {
     float* C = a.whole ? a.g.C : a.g.partial + (int64_t)slice * a.g.M * a.g.N;
     const int64_t ldc = a.whole ? a.g.ldc : a.g.N;
     const float* bias = a.whole ? a.g.bias : nullptr;
-    // Elements from where a row of C2 would lie in C to where it lies.
-    const int64_t away = a.whole && a.g.C2 ? (int64_t)(reinterpret_cast<intptr_t>(a.g.C2) - reinterpret_cast<intptr_t>(C)) / 4 - a.g.rows * ldc : 0;
-    const int64_t second = a.whole && a.g.C2 ? a.g.rows : a.g.M;
-    const bool vec = ldc % 4 == 0 && reinterpret_cast<uintptr_t>(C) % 16 == 0 && away % 4 == 0;
+    const bool both = OUT == TO_BOTH && a.whole;
+    const bool vec = ldc % 4 == 0 && reinterpret_cast<uintptr_t>(C) % 16 == 0 &&
+                     (!both || reinterpret_cast<uintptr_t>(a.g.C2) % 16 == 0);
     const int64_t mw = m0 + wm * (TM / 2) + n2, nw = n0 + wn * (TN / 2) + 4 * hh2;
     if (a.whole && a.g.add) {  // all of C's loads ahead of the stores
 #pragma unroll
@@ -516,14 +518,14 @@ __global__ __launch_bounds__(256 * KW, 3) void gemm_f32_kernel(Args a) {
             for (int q = 0; q < 4; ++q) {
                 const int64_t c0 = nw + 32 * j + 8 * q;
                 f32x4 o{acc[j][k][4 * q], acc[j][k][4 * q + 1], acc[j][k][4 * q + 2], acc[j][k][4 * q + 3]};
-                if constexpr (EPI) {
+                if constexpr (OUT == TO_EPILOGUE) {
                     if (a.whole) {
                         float v[4] = {o[0], o[1], o[2], o[3]};
                         if (c0 < a.g.N) run_epilogue<4>(a.g, m, c0, v);
                         continue;
                     }
                 }
-                float* d = C + m * ldc + (m < second ? 0 : away) + c0;
+                float* d = (both && m >= a.g.rows ? a.g.C2 + (m - a.g.rows) * ldc : C + m * ldc) + c0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (bias && c0 + e < a.g.N) o[e] += bias[c0 + e];
@@ -538,8 +540,8 @@ __global__ __launch_bounds__(256 * KW, 3) void gemm_f32_kernel(Args a) {
     }
 }
 
-// C (+)= the slices' partial products in slice order, + bias (EPI: and the linear layer's epilogue).
-template <int VEC, bool EPI>
+// C (+)= the slices' partial products in slice order, + bias (and the epilogue).
+template <int VEC, int OUT>
 __global__ __launch_bounds__(256) void gemm_f32_reduce(Args a) {
     typedef float V __attribute__((ext_vector_type(VEC)));
     const int64_t MN = a.g.M * a.g.N, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
@@ -548,14 +550,14 @@ __global__ __launch_bounds__(256) void gemm_f32_reduce(Args a) {
     V sum = *reinterpret_cast<const V*>(a.g.partial + i);
 #pragma unroll 8
     for (int s = 1; s < a.slices; ++s) sum += *reinterpret_cast<const V*>(a.g.partial + s * MN + i);
-    if constexpr (EPI) {
+    if constexpr (OUT == TO_EPILOGUE) {
         float v[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = sum[e];
         run_epilogue<VEC>(a.g, m, n, v);
         return;
     }
-    float* d = a.g.C2 && m >= a.g.rows ? a.g.C2 + (m - a.g.rows) * a.g.ldc + n : a.g.C + m * a.g.ldc + n;
+    float* d = (OUT == TO_BOTH && m >= a.g.rows ? a.g.C2 + (m - a.g.rows) * a.g.ldc : a.g.C + m * a.g.ldc) + n;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) d[e] = sum[e] + (a.g.bias ? a.g.bias[n + e] : 0.f) + (a.g.add ? d[e] : 0.f);
 }
@@ -611,23 +613,26 @@ void launch_t(const Args& a, hipStream_t st) {
     const bool ta = a.g.terms[0].ta != 0, tb = a.g.terms[0].tb != 0;
     if (with_epilogue(a.g)) {
         if (tb)
-            hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, true, true>), grid, dim3(256 * KW), 0, st, a);
+            hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, true, TO_EPILOGUE>), grid, dim3(256 * KW), 0, st, a);
         else
-            hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, false, true>), grid, dim3(256 * KW), 0, st, a);
-    } else if (ta && tb)
-        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, true, true, false>), grid, dim3(256 * KW), 0, st, a);
+            hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, false, TO_EPILOGUE>), grid, dim3(256 * KW), 0, st, a);
+    } else if (a.g.C2)
+        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, true, false, TO_BOTH>), grid, dim3(256 * KW), 0, st, a);
+    else if (ta && tb)
+        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, true, true, TO_C>), grid, dim3(256 * KW), 0, st, a);
     else if (ta)
-        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, true, false, false>), grid, dim3(256 * KW), 0, st, a);
+        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, true, false, TO_C>), grid, dim3(256 * KW), 0, st, a);
     else if (tb)
-        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, true, false>), grid, dim3(256 * KW), 0, st, a);
+        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, true, TO_C>), grid, dim3(256 * KW), 0, st, a);
     else
-        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, false, false>), grid, dim3(256 * KW), 0, st, a);
+        hipLaunchKernelGGL((gemm_f32_kernel<T, BK, KW, false, false, TO_C>), grid, dim3(256 * KW), 0, st, a);
 }
 
 template <int VEC> void launch_reduce(const Args& a, hipStream_t st) {
     const dim3 grid((unsigned)((a.g.M * a.g.N / VEC + 255) / 256));
-    if (with_epilogue(a.g)) hipLaunchKernelGGL((gemm_f32_reduce<VEC, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((gemm_f32_reduce<VEC, false>), grid, dim3(256), 0, st, a);
+    if (with_epilogue(a.g)) hipLaunchKernelGGL((gemm_f32_reduce<VEC, TO_EPILOGUE>), grid, dim3(256), 0, st, a);
+    else if (a.g.C2) hipLaunchKernelGGL((gemm_f32_reduce<VEC, TO_BOTH>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((gemm_f32_reduce<VEC, TO_C>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -640,7 +645,7 @@ size_t gemm_f32_workspace(const GemmF32& g) {
 hipError_t launch_gemm_f32(const GemmF32& g, hipStream_t st) {
     if (g.M <= 0 || g.N <= 0) return hipSuccess;
     if (with_epilogue(g) && (g.ldc != g.N || g.terms[0].ta || g.add || g.C2)) return hipErrorInvalidValue;
-    if (g.C2 && g.add) return hipErrorInvalidValue;
+    if (g.C2 && (g.add || !g.terms[0].ta || g.terms[0].tb)) return hipErrorInvalidValue;
     const Plan p = plan(g);
     if (p.small)
         launch_t<64, 32, 2>(p.a, st);
