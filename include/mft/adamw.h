@@ -17,9 +17,9 @@
  *
  *   scale = max(max |x| / 448, 2^-126),  q = e4m3(x / scale) to nearest even
  *
- * (both quotients rounded to fp32) for x = m and x = sqrt(v), a positive sqrt(v) being at least the smallest number
- * 2^-9 (as zero it would leave m / eps of the next step).  p is stepped with m
- * and v as they are before that.
+ * (both quotients rounded to fp32) for x = m and x = sqrt(v), a positive sqrt(v)
+ * being at least the smallest number 2^-9 (as zero it would leave m / eps of the
+ * next step).  p is stepped with m and v as they are before that.
  *
  * All arithmetic is in fp32, the norm and the powers of beta in 64 bits.  A
  * gradient that is no number makes its p, m and v (in 8 bits: its 256 states)

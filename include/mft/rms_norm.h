@@ -12,10 +12,10 @@
  *
  *   scale = max(max |y| / 448, 2^-126),  q = e4m3(y / scale) to nearest even
  *
- * with both quotients rounded to fp32.
- * A row with an infinity or a NaN has no numbers (its q are NaN, or 0 where y is
- * finite in a row with an infinity).  MFT_NORM_NONE holds s itself so: the form
- * in which mft/gated_linear.h takes activations and weights in 8 bits.
+ * with both quotients rounded to fp32.  A row with an infinity or a NaN has no
+ * numbers (its q are NaN, or 0 where y is finite in a row with an infinity).
+ * MFT_NORM_NONE holds s itself so: the form in which mft/gated_linear.h takes
+ * activations and weights in 8 bits.
  *
  * Backward, with h = s * rstd and g = dy * f:
  *

@@ -37,8 +37,8 @@ class AdamW:
     state: {"step": int64 [], "exp_avg", "exp_avg_sq": flat, "exp_avg_scale",
     "exp_avg_sq_scale": with 8 bits, "master": fp32, of the bf16 parameters}.  In
     the flat ones each parameter's part starts at a multiple of 256 values
-    (views()).  One step's number serves all parameters, also one that had no
-    gradient in some steps."""
+    (views()); state_dict() says whose they are.  One step's number serves all
+    parameters, also one that had no gradient in some steps."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
         self.params = list(params)

@@ -70,9 +70,10 @@ mft::GemmF32 f_fwd(const mft_gated_linear_desc* d) {
     return g;
 }
 // fp32: dx along both halves of dz as one product, with the weights laid beside one
-// another, or as two, the second added to the first.  509 x 640 -> 2048 36 us and 6
-// for the copy against 45; copying larger weights costs more than the second launch's
-// start.
+// another, or as two, the second added to the first: the copy costs less than the second
+// launch's start and end up to about 4 M weights, and more beyond (the limit stays clear of that).  dx alone, copied and
+// added, us, weights [ff, in]: 509 x 640 -> 2048 45 and 51, 2048 rows 95 and 109; 509 x 1024 ->
+// 2048 50 and 62; 509 x 896 -> 4864 86 and 90; 128 x 1152 -> 6912 66 and 55, 2048 rows 602 and 587.
 constexpr int64_t kJoinedWeight = int64_t(1) << 21;
 bool f_joins(const mft_gated_linear_desc* d) { return d->in_dim * d->ff_dim <= kJoinedWeight; }
 mft::GemmF32 f_dx(const mft_gated_linear_desc* d) {
@@ -106,8 +107,9 @@ FwdLayout fwd_layout(const mft_gated_linear_desc* d) {
     l.total = l.gemm + mft::gemm_f32_workspace(f_fwd(d));
     return l;
 }
-// fp32: one product for both weights' gradients stored [ff, in], each to its own memory.  Twice the tiles at once: 509 x 640 -> 2048 31 us against 45 (bf16 at 4096 x 1152 -> 6912, whose single products fill the
-// GPU: 341 us of a backward against 338).
+// fp32: one product for both weights' gradients stored [ff, in], each to memory of its own.  Twice the tiles at
+// once: 509 x 640 -> 2048 31 us against 45 (bf16 at 4096 x 1152 -> 6912, whose single products fill the GPU: 341 us
+// of a backward against 338).
 bool may_be_both(const mft_gated_linear_desc* d) { return !is_bf(d) && d->w_transposed; }
 
 struct BwdLayout {

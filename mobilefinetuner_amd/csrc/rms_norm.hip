@@ -6,7 +6,7 @@
 // residual are read once, the sum s = x + residual is rounded to the stream's
 // type, stored and normed as it is stored, so that the backward's s is the
 // forward's.  Longer rows go by memory.  All of it is bound by memory: 8192 x 1152 in
-// bf16 with a residual and into 8 bits 17.4 us (3.8 TB/s; a copy reaches 4.75).
+// bf16 with a residual and into 8 bits 17.0 us (3.9 TB/s; a copy reaches 4.75).
 //
 // Backward: the row's sum of g h gives dx in one pass over s, dy and the
 // stream's gradient.  The sums over rows, dw, stay in registers: a workgroup takes
@@ -207,8 +207,8 @@ template <int WPR> constexpr int kBwdThreads = WPR == 1 ? 512 : 64 * WPR;
 // Workgroup g: rows in steps of groups * (rows a workgroup holds at once).  EVEN:
 // D is a multiple of the vector, so that no element is looked at by itself.  A row
 // stays in T between its two passes, over the sum and to dx: 16384 x 1152 in bf16 with
-// the stream's gradient 36 us (4.2 TB/s); in fp32 its registers leave eight waves to a
-// CU, 56 us.
+// the stream's gradient 34 us (4.4 TB/s); held as fp32 numbers, whose registers leave
+// eight waves to a CU, it took 56.
 template <typename T, int WPR, int CH, bool PARAMS, bool EVEN>
 __global__ __launch_bounds__(kBwdThreads<WPR>, WPR == 4 ? 2 : 4) void rms_bwd(RmsNormArgs a) {
     constexpr int V = kVec<T>, TPR = 64 * WPR, NT = kBwdThreads<WPR>, RPB = NT / TPR;
@@ -389,9 +389,10 @@ Shape bwd_shape(int64_t D, int vec) {
     return {0, 0};
 }
 // Workgroups of the backward, each of which leaves a partial.  One to a CU, or two of
-// four waves from eight rows a CU on: 4096 x 1152 in fp32 18 us (one: 22), 1001 x 1153 12
-// (11); of eight waves a row each, 16384 x 1152 in bf16 36 (two: 38, four: 39), of
-// sixteen, 2048 x 8192 33 (two: 37).
+// four waves from eight rows a CU on: 4096 x 1152 in fp32 23 us (one: 27, four: 22), 8192 x
+// 2304 in bf16 40 (52, 38), while 1001 x 1153 in fp32 waits for the host either way; of eight
+// waves a row each, 16384 x 1152 in bf16 36 (two: 37, four: 39), of sixteen, 2048 x 8192
+// 33 (37, 43).  Calls over operands out of cache, with dtotal.
 int64_t bwd_groups(int64_t N, int64_t D, int vec) {
     const Shape s = bwd_shape(D, vec);
     const int64_t at_once = s.wpr == 1 ? 8 : 1, cus = device_cus();
