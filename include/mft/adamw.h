@@ -17,7 +17,7 @@
  *
  *   scale = max(max |x| / 448, 2^-126),  q = e4m3(x / scale) to nearest even
  *
- * (both quotients rounded to fp32) for x = m and x = sqrt(v), a positive sqrt(v)
+ * (as mft/rms_norm.h rounds them) for x = m and x = sqrt(v), a positive sqrt(v)
  * being at least the smallest number 2^-9 (as zero it would leave m / eps of the
  * next step).  p is stepped with m and v as they are before that.
  *

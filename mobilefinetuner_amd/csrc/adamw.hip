@@ -3,7 +3,7 @@
 // Bound by memory: in fp32 28 bytes a value (the gradient and three values read,
 // three written), with 8-bit states and a bf16 parameter 16.  A block's 27 M values in
 // fp32 127 us (6.0 TB/s, part of it from the last-level cache) and 36 for the sums of
-// squares; a bf16 table of 168 M with 8-bit states 498 us (5.4 TB/s).
+// squares; a bf16 table of 168 M with 8-bit states 493 us (5.5 TB/s).
 //
 // The tensors are cut into chunks of whole groups of 256 values, a workgroup to a
 // chunk.  A launch's tensors lie in its arguments, which the host fills and a
@@ -163,13 +163,15 @@ __global__ __launch_bounds__(kStepThreads) void adamw_factors(StepArgs a) {
     *a.f = f;
 }
 
-// One value's step.
+// One value's step.  The averages are rounded as by torch's multi-tensor operations (the state times beta, then the
+// gradient's share with one rounding): with the gradient's product rounded first 400 of 168 M 8-bit numbers of a step
+// came out one off, where a quotient is halfway between two, and now and then a scale of the next step by percents.
 template <int BITS>
 __device__ __forceinline__ void update(const Args<BITS>& a, const Factors& f, float keep, float g, float& p, float& m,
                                        float& v, float& root) {
     g *= f.clip;
-    m = fmaf(a.beta1, m, a.rest1 * g);
-    v = fmaf(a.beta2, v, a.rest2 * g * g);
+    m = fmaf(a.rest1, g, a.beta1 * m);
+    v = fmaf(a.rest2 * g, g, a.beta2 * v);
     root = sqrtf(v);
     p = fmaf(p, keep, -f.step_size * (m / fmaf(root, f.root, a.eps)));
 }

@@ -14,9 +14,10 @@ constexpr float kE4m3Max = 448.f, kE4m3Min = 0x1p-9f;
 constexpr float kScaleMin = 0x1p-126f;  // a scale's reciprocal stays finite
 
 // The scale that takes a maximum of magnitudes (its bits; a NaN's are above
-// infinity's, so it stays) to the largest e4m3 number.
+// infinity's, so it stays) to the largest e4m3 number: times 1 / 448 in fp32, as
+// torch's kernels divide by a number, so that both hold the same numbers.
 __device__ __forceinline__ float e4m3_scale(uint32_t max_bits) {
-    const float s = __uint_as_float(max_bits) / kE4m3Max;
+    const float s = __uint_as_float(max_bits) * (1.0f / kE4m3Max);
     return s < kScaleMin ? kScaleMin : s;  // a NaN stays
 }
 
@@ -46,7 +47,7 @@ struct E4m3Divisor {
     }
 };
 
-// Four values to nearest even.  Up to 448 (1 + 2^-23), which rounds to 448: no
+// Four values to nearest even.  Up to 448 (1 + 2^-22), which rounds to 448: no
 // value of a group exceeds its scale's by more.
 __device__ __forceinline__ uint32_t e4m3_pack4(float a, float b, float c, float d) {
     int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);

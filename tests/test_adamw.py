@@ -547,7 +547,7 @@ def test_nothing_but_empty_gradients(dev, bits):
 
 @pytest.mark.gpu
 def test_eight_bits_are_those_of_the_quotient(dev):
-    """To the bit, scale = max |x| / 448 and q = e4m3(x / scale), both quotients in fp32, for x = m and sqrt(v): those
+    """To the bit, scale = max |x| (1 / 448) and q = e4m3(x / scale), all in fp32, for x = m and sqrt(v): those
     of a first step are (1 - beta1) g and sqrt((1 - beta2) g^2), as with states in 32 bits.  Gradients with few
     digits, whose quotients often lie halfway between two numbers."""
     from mobilefinetuner_amd.adamw import AdamW
@@ -563,7 +563,7 @@ def test_eight_bits_are_those_of_the_quotient(dev):
     wide, narrow = (o.state for o in opts)
     for name, x in (("exp_avg", wide["exp_avg"].cpu()), ("exp_avg_sq", wide["exp_avg_sq"].cpu().sqrt())):
         x = x.view(-1, 256)
-        scale = x.abs().amax(1) / torch.tensor(448.0)
+        scale = x.abs().amax(1) * (torch.tensor(1.0) / 448)
         assert torch.equal(narrow[name + "_scale"].cpu(), scale)
         q = (x / scale[:, None]).to(torch.float8_e4m3fn).float()
         if name == "exp_avg_sq":
@@ -629,3 +629,39 @@ def test_weight_decay_set_between_steps(dev):
         with pytest.raises(ValueError, match="weight_decay has"):
             opt.step()
     assert int(opt.state["step"]) == t and all(torch.equal(a[k], b[k]) for a, b in zip(before, snapshot(opt)) for k in "pmv")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_eight_bits_of_several_steps(dev, dtype):
+    """To the bit, over five steps: beta times the state rounded, then the gradient's share added with one rounding (in
+    64 bits here, whose own rounding comes before that in one of 2^29), then numbers and scales as above.  A
+    number off at a tie would move its group's scale by percents in a step after it."""
+    from mobilefinetuner_amd.adamw import AdamW
+    n = 1 << 22
+    g = torch.Generator(device=dev).manual_seed(22)
+    p = (0.02 * torch.randn(n, device=dev, generator=g)).to(dtype).requires_grad_(True)
+    opt = AdamW([p], LR, BETAS, EPS, state_bits=8)
+    m, v = torch.zeros(n, device=dev), torch.zeros(n, device=dev)
+    b1, b2, r1, r2 = (torch.tensor(x, device=dev) for x in (*BETAS, 1 - BETAS[0], 1 - BETAS[1]))
+    by_448 = torch.tensor(1.0, device=dev) / torch.tensor(448.0, device=dev)
+
+    def held(x, positive):
+        x = x.view(-1, 256)
+        scale = (x.abs().amax(1) * by_448).clamp(min=2.0 ** -126)
+        q = x / scale[:, None]
+        q = (torch.where(q > 0, q.clamp(min=2.0 ** -9), q) if positive else q).to(torch.float8_e4m3fn).float()
+        return q, scale, (q * scale[:, None]).view(-1)
+
+    for _ in range(5):
+        p.grad = (1e-3 * torch.randn(n, device=dev, generator=g)).to(dtype)
+        opt.step()
+        grad = p.grad.float()
+        m = ((b1 * m).double() + r1.double() * grad.double()).float()
+        v = ((b2 * v).double() + (r2 * grad).double() * grad.double()).float()
+        mq, ms, m = held(m, False)
+        vq, vs, root = held(v.sqrt(), True)
+        v = root.square()
+        for name, q, scale in (("exp_avg", mq, ms), ("exp_avg_sq", vq, vs)):
+            assert torch.equal(opt.state[name + "_scale"], scale)
+            assert torch.equal(opt.state[name].float().view(-1, 256), q)

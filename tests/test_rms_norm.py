@@ -528,9 +528,10 @@ def test_operands_that_do_not_fit_refused(dev):
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("D", [64, 1152, 1153, 4100, 20000, 70000])
 def test_eight_bits_are_those_of_the_quotient(dev, D, dtype):
-    """To the bit, scale = max / 448 and q = e4m3(x / scale), both quotients in fp32: those of bf16 rows often lie
+    """To the bit, scale = max (1 / 448) and q = e4m3(x / scale), all in fp32: the quotients of bf16 rows often lie
     halfway between two numbers, where one by a reciprocal comes out on the other side.  From the smallest
-    scales to the largest; a kernel for each count of waves, and one by memory."""
+    scales to the largest; a kernel for each count of waves, and one by memory.  torch's own operations on the GPU
+    give the same."""
     from mobilefinetuner_amd import rms_norm as L
     g = torch.Generator().manual_seed(D)
     x = (torch.randn(max(7, 400000 // D), D, generator=g) * 2.0 ** -7).to(DT[dtype])
@@ -539,6 +540,8 @@ def test_eight_bits_are_those_of_the_quotient(dev, D, dtype):
     print(f"[case] {list(x.shape)} {dtype}", flush=True)
     q, scale = L.quantize_rows(x.to(dev))
     up = x.float()
-    want = (up.abs().amax(1) / torch.tensor(448.0)).clamp(min=2.0 ** -126)
+    want = (up.abs().amax(1) * (torch.tensor(1.0) / 448)).clamp(min=2.0 ** -126)
     assert torch.equal(scale.cpu(), want)
     assert torch.equal(q.float().cpu(), (up / want[:, None]).to(torch.float8_e4m3fn).float())
+    own = (up.to(dev).abs().amax(1) / 448.0).clamp(min=2.0 ** -126)
+    assert torch.equal(own, scale) and torch.equal((up.to(dev) / own[:, None]).to(torch.float8_e4m3fn).float(), q.float())
