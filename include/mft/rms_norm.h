@@ -13,8 +13,9 @@
  *   scale = max(max |y| / 448, 2^-126),  q = e4m3(y / scale) to nearest even
  *
  * the division by 448 being a product by the fp32 number next to 1 / 448 (as torch's
- * kernels have it), and y / scale rounded to fp32 first.  A row with an infinity or a NaN has no
- * numbers (its q are NaN, or 0 where y is finite in a row with an infinity).
+ * kernels have it), and y / scale rounded to fp32 first.  A row with an infinity
+ * or a NaN has no numbers (its q are NaN, or 0 where y is finite in a row with an
+ * infinity).
  * MFT_NORM_NONE holds s itself so: the form in which mft/gated_linear.h takes
  * activations and weights in 8 bits.
  *
